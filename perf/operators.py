@@ -363,7 +363,7 @@ def run(state):
 def e4m3(v):
     """the nearest value with four significant bits, an exponent of -6 at least and a size of 448 at most (ties to the even one)"""
     _, e = torch.frexp(v)
-    step = torch.ldexp(torch.ones_like(v), e.clamp_min(-5) - 4)
+    step = ((e.clamp_min(-5) - 4 + 1023).long() << 52).view(torch.float64)          # (2^(e - 4), exactly)
     return (torch.round(v / step) * step).clamp(-448.0, 448.0)
 
 
