@@ -833,6 +833,41 @@ int ifa_moe_experts_routed_rows_f32(int score_kind, int renorm, float renorm_eps
                                     int accumulate, ifa_stream stream);
 
 /* ======================================================================== */
+/* A feed-forward in 8-bit floating point (csrc/ifa_fp8_rows.hip, ifa_linear_fp8.hip, ifa_moe_fp8.hip).  Values are e4m3 bytes (four significant     */
+/* bits, largest value 448).  Activation rows have a fp32 scale for each 128 columns ([rows][lds], lds >= ceil(cols / 128)), matrices              */
+/* [rows][cols] (row-major, no padding) one for each 128 x 128 block ([ceil(rows / 128)][ceil(cols / 128)]); the last block of either may be a part   */
+/* of one.  Columns come in whole 16s, e4m3 rows start on 16 bytes.  A block's scale is max(max |v| / 448, 2^-126), its values e4m3(v / scale)        */
+/* (to nearest, ties to even; v times the 32-bit reciprocal of the scale).  A block that holds an infinity or a NaN stands for NaN in all its values. */
+/* Dtypes of rows that are not quantised: IFA_F32, IFA_F16 or IFA_BF16.  Sums, norms and activations are fp32.  Deterministic.                       */
+/* ======================================================================== */
+/* residual update, RMS norm and quantisation in one pass: x += m (m null: x as it is; the sum rounded to dtype), v = x / sqrt(mean(x^2) + eps) * (w_offset + w[c])
+ * (w bf16 [cols], null: 0), (q, scale) = v quantised, h = v in dtype (nullable: what a router reads).  x, m and h [rows][ld*] of dtype, whole 16 bytes a row;
+ * x, m and h are different buffers.  cols <= 32768. */
+int ifa_norm_add_fp8(int dtype, void *x, size_t ldx, size_t rows, size_t cols, const void *m, size_t ldm, const void *w_bf16, float w_offset, float eps, void *h, size_t ldh,
+                     void *q_e4m3, size_t ldq, void *scale_f32, size_t lds, ifa_stream stream);
+/* gated activation and quantisation: rows gate | up of 2 cols values, v = f(gate, up), kinds 0 / 1 / 2 / 3 as ifa_glu_ex_f32; kind 4: rows of cols values as they are */
+int ifa_glu_fp8(int kind, float limit, int dtype, const void *gate_up, size_t ld, size_t rows, size_t cols, void *q_e4m3, size_t ldq, void *scale_f32, size_t lds, ifa_stream stream);
+/* C[t][n] (+)= sum_b a_scale[t][b] w_scale[n / 128][b] (sum over block b of a[t][k] w[n][k]) + bias[n]; bias bf16 [rows] nullable; accumulate != 0 adds into C (the sum
+ * rounded once to c_dtype).  Workspace: ifa_linear_fp8_workspace_bytes (a product without one, or with less, is the same but may be slower). */
+size_t ifa_linear_fp8_workspace_bytes(size_t rows, size_t cols, size_t tokens);
+int ifa_linear_fp8(const void *w_e4m3, const void *w_scale_f32, size_t rows, size_t cols, const void *a_e4m3, size_t lda, const void *a_scale_f32, size_t lds, size_t tokens,
+                   const void *bias_bf16, int accumulate, int c_dtype, void *c, size_t ldc, void *ws, size_t ws_bytes, ifa_stream stream);
+/* Router that chooses by groups: the n_all experts (at most 1024) are `groups` (at most 64) equal ranges.  score = softmax (score_kind 0) or sigmoid (1) of the logits, choice =
+ * score + correction[e] (fp32: a bias for balance moves in steps that a bfloat16 would lose; nullable); a group's value is the sum of its group_best (1 or 2) largest choices; the
+ * groups_kept groups of largest value stay; of their experts the `top` (at most 64) largest choices are taken, in falling order, the lower index first on ties.  weight = score,
+ * renorm != 0: score / (sum of the taken scores + renorm_eps) (0 if that is 0), times wgt_scale.  An expert whose logit is -inf or NaN (or whose choice is NaN) is never taken and adds
+ * nothing to its group; what is left over of a row has idx -1 and weight 0.  Scores and choices are formed and compared in 64 bits.  idx_dev / wgt_f32: [rows][top]. */
+int ifa_moe_route_groups_f32(int score_kind, int groups, int groups_kept, int group_best, int renorm, float renorm_eps, float wgt_scale, const void *logits_f32, size_t ld, size_t rows, int n_all,
+                             int top, const void *correction_f32, int *idx_dev, void *wgt_f32, ifa_stream stream);
+/* Gated experts over quantised rows: y[t] (+)= sum_k wgt[t][k] * Down_e q(f(Gate_e a[t], Up_e a[t])), e = idx[t][k], f as ifa_glu_fp8 (kinds 0 .. 3), q: quantised as above.  gate_up
+ * [experts][gate ff | up ff][width] with scales [experts][2][ceil(ff / 128)][ceil(width / 128)], down [experts][width][ff] with scales [experts][ceil(width / 128)][ceil(ff / 128)].
+ * idx outside 0 .. experts - 1 adds nothing; an expert may come more than once in a row.  width and ff in whole 16s. */
+size_t ifa_moe_experts_fp8_workspace_bytes(size_t rows, int top, int width, int ff, int experts);
+int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t lda, const void *a_scale_f32, size_t lds, size_t rows, int width, int ff, int experts, int top,
+                        const void *gate_up_e4m3, const void *gate_up_scale_f32, const void *down_e4m3, const void *down_scale_f32, const int *idx_dev, const void *wgt_f32, void *ws,
+                        size_t ws_bytes, int y_dtype, void *y, size_t ldy, int accumulate, ifa_stream stream);
+
+/* ======================================================================== */
 /* Layer-list worker: a decoder whose layers are given one by one, each with its own sequence mixer, a 32-bit residual       */
 /* stream and bfloat16 weights (csrc/ifa_engine_layered.hip).  It is an ifa_model: finalize / kv_slots / select_kv /        */
 /* forward / decode / decode_batch / set_option / set_excluded_tokens / get_buffer / destroy work as above (a "KV slot" holds */

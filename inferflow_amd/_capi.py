@@ -230,6 +230,13 @@ SIGNATURES = {
     "ifa_linear_bf16w_act": (_i, [_vp, _sz, _sz, _vp, _sz, _sz, _vp, _i, _i, _vp, _sz, _vp]),
     "ifa_moe_route_renorm_f32": (_i, [_i, _i, _f, _f, _vp, _sz, _sz, _i, _i, _vp, _vp, _vp, _vp]),
     "ifa_moe_route_rows_renorm_f32": (_i, [_i, _i, _f, _f, _vp, _sz, _sz, _i, _vp, _i, _i, _vp, _vp, _vp, _vp]),
+    "ifa_norm_add_fp8": (_i, [_i, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _f, _f, _vp, _sz, _vp, _sz, _vp, _sz, _vp]),
+    "ifa_glu_fp8": (_i, [_i, _f, _i, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _sz, _vp]),
+    "ifa_linear_fp8_workspace_bytes": (_sz, [_sz, _sz, _sz]),
+    "ifa_linear_fp8": (_i, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _sz, _vp, _i, _i, _vp, _sz, _vp, _sz, _vp]),
+    "ifa_moe_route_groups_f32": (_i, [_i, _i, _i, _i, _i, _f, _f, _vp, _sz, _sz, _i, _i, _vp, _vp, _vp, _vp]),
+    "ifa_moe_experts_fp8_workspace_bytes": (_sz, [_sz, _i, _i, _i, _i]),
+    "ifa_moe_experts_fp8": (_i, [_i, _f, _vp, _sz, _vp, _sz, _sz, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i, _vp, _sz, _i, _vp]),
     "ifa_model_create_layered": (_i, [_vp, _vp, C.POINTER(_vp)]),
     "ifa_model_set_tensor_host": (_i, [_vp, _i, _i, _i, _vp, _sz, _sz]),
     "ifa_model_logits_f32": (_i, [_vp, C.POINTER(_vp), C.POINTER(_sz), C.POINTER(_sz)]),

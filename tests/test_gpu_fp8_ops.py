@@ -1,0 +1,490 @@
+"""The operators of a feed-forward in 8-bit floating point through the C ABI against their formulas in 64 bits (tests/fp8_oracle.py): sizes that end inside a
+block or a tile, strides, all types, blocks of zeros and of tiny values, infinities and NaN, empty choices, ties, far offsets, streams and graphs."""
+import math
+
+import pytest
+import torch
+
+import inferflow_amd as ia
+from tests import fp8_oracle as orc
+from tests.gpu_util import capi, p, sync
+
+pytestmark = pytest.mark.gpu
+
+F8 = orc.F8
+TYPES = {0: torch.float32, 1: torch.float16, 2: torch.bfloat16}
+HALF_STEP = {0: 2.0 ** -24, 1: 2.0 ** -11, 2: 2.0 ** -8}
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def padded(v, ld, fill):
+    """v's rows in a buffer of stride ld"""
+    out = torch.full((v.shape[0], ld), fill, dtype=torch.float32, device="cuda").to(v.dtype)
+    out[:, :v.shape[1]] = v
+    return out
+
+
+def codes(rows, ld):
+    return torch.full((rows, ld), 0x55, dtype=torch.uint8, device="cuda")
+
+
+def here():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def norm(dtype, x, m, w, off, eps, cols, h, q, scale):
+    ia.check(capi().ifa_norm_add_fp8(dtype, p(x), x.shape[1], x.shape[0], cols, p(m), m.shape[1] if m is not None else 0, p(w), off, eps, p(h), h.shape[1] if h is not None else 0, p(q), q.shape[1],
+                                     p(scale), scale.shape[1], here()))
+
+
+def glu(kind, dtype, gu, cols, q, scale, limit=7.0):
+    ia.check(capi().ifa_glu_fp8(kind, limit, dtype, p(gu), gu.shape[1], gu.shape[0], cols, p(q), q.shape[1], p(scale), scale.shape[1], here()))
+
+
+def linear(w, sw, a, sa, tokens, cols, bias, accumulate, dtype, c, ws=None):
+    ia.check(capi().ifa_linear_fp8(p(w), p(sw), w.shape[0], cols, p(a), a.shape[1], p(sa), sa.shape[1], tokens, p(bias), accumulate, dtype, p(c), c.shape[1], p(ws), 0 if ws is None else ws.numel(),
+                                   here()))
+
+
+def room(rows, cols, tokens):
+    n = capi().ifa_linear_fp8_workspace_bytes(rows, cols, tokens)
+    return torch.full((max(n, 16),), 0xFF, dtype=torch.uint8, device="cuda")
+
+
+def route(score, groups, kept, best, renorm, eps, scale, z, corr, top, ld=None):
+    rows, n = z.shape
+    idx, wgt = torch.full((rows, top), 77, dtype=torch.int32, device="cuda"), torch.full((rows, top), 77.0, device="cuda")
+    zd = z.cuda() if ld is None else padded(z.cuda(), ld, 50.0)
+    ia.check(capi().ifa_moe_route_groups_f32(score, groups, kept, best, int(renorm), eps, scale, p(zd), zd.shape[1], rows, n, top, p(None if corr is None else corr.cuda()), p(idx), p(wgt), here()))
+    return idx, wgt
+
+
+def experts(kind, a, sa, width, gu, sgu, down, sdown, idx, wgt, dtype, y, accumulate, limit=7.0):
+    E, _, ff, _ = gu.shape
+    rows, top = idx.shape
+    ws = torch.full((capi().ifa_moe_experts_fp8_workspace_bytes(rows, top, width, ff, E),), 0xFF, dtype=torch.uint8, device="cuda")
+    ia.check(capi().ifa_moe_experts_fp8(kind, limit, p(a), a.shape[1], p(sa), sa.shape[1], rows, width, ff, E, top, p(gu), p(sgu), p(down), p(sdown), p(idx), p(wgt), p(ws), ws.numel(), dtype, p(y),
+                                        y.shape[1], accumulate, here()))
+
+
+# ---------------------------------------------------------------- rows in 8 bits
+# A row's sum of squares is off by at most (values a thread adds one after the other: 32, lanes and waves: 22) halves of a unit, its root by half of that; five roundings behind it.
+NORM_ERR = ((32 + 22) / 2 + 8) * 2.0 ** -24
+
+
+def check_quantised(q, scale, v, rel):
+    """q and scale against exact rows v, each value known to a relative error rel"""
+    cols = v.shape[1]
+    s = orc.scales(v)
+    assert ((scale.double() - s).abs() <= (rel + 2.0 ** -23) * s).all()
+    f = orc.per_column(scale, cols)
+    x = v / f
+    assert orc.between(q.view(F8).double(), x, x.abs() * (rel + 3 * 2.0 ** -24)).all()
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("rows,cols", [(1, 16), (3, 48), (2, 128), (5, 144), (1, 1040), (7, 2048), (2, 4112), (3, 8208), (1, 16400), (2, 32768), (300, 256), (33, 2832)])
+@pytest.mark.parametrize("add,plain,weight", [(True, True, True), (False, False, True), (True, False, False)])
+def test_norm_with_the_residual(dtype, rows, cols, add, plain, weight):
+    g, kind = gen(rows * 7 + cols), TYPES[dtype]
+    x0 = (torch.randn(rows, cols, generator=g, device="cuda") * torch.exp(2 * torch.randn(rows, 1, generator=g, device="cuda"))).to(kind)
+    m0 = torch.randn(rows, cols, generator=g, device="cuda").to(kind)
+    w = (0.2 * torch.randn(cols, generator=g, device="cuda")).to(torch.bfloat16)
+    x, m = padded(x0, cols + 16, 9.0), padded(m0, cols + 32, math.nan)
+    h = padded(torch.zeros_like(x0), cols + 8, 5.0) if plain else None
+    q, scale = codes(rows, cols + 48), torch.full((rows, orc.blocks(cols) + 3), 3.0, device="cuda")
+    norm(dtype, x, m if add else None, w if weight else None, 1.0, 1e-5, cols, h, q, scale); sync()
+    want = (x0.float() + m0.float()).to(kind) if add else x0
+    assert torch.equal(x[:, :cols], want) and (x[:, cols:] == 9.0).all()
+    d = want.double()
+    v = d / torch.sqrt(d.square().mean(-1, keepdim=True) + 1e-5) * (1.0 + (w.double() if weight else 0.0))
+    check_quantised(q[:, :cols].contiguous(), scale[:, :orc.blocks(cols)], v, NORM_ERR)
+    assert (q[:, cols:] == 0x55).all() and (scale[:, orc.blocks(cols):] == 3.0).all()
+    if plain:
+        assert ((h[:, :cols].double() - v).abs() <= (NORM_ERR + HALF_STEP[dtype]) * v.abs() + (2.0 ** -25 if dtype == 1 else 0.0)).all() and (h[:, cols:] == 5.0).all()
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("kind", [0, 1, 2, 3, 4])
+@pytest.mark.parametrize("rows,cols", [(1, 16), (2, 112), (3, 128), (5, 272), (130, 64), (9, 2832), (2, 40000)])
+def test_activation(dtype, kind, rows, cols):
+    g = gen(kind * 100 + rows + cols)
+    v0 = (3 * torch.randn(rows, cols * (1 if kind == 4 else 2), generator=g, device="cuda")).to(TYPES[dtype])
+    gu = padded(v0, v0.shape[1] + 24, math.nan)
+    q, scale = codes(rows, cols + 16), torch.full((rows, orc.blocks(cols) + 1), 3.0, device="cuda")
+    glu(kind, dtype, gu, cols, q, scale); sync()
+    d = v0.double()
+    v = orc.gated(kind, d[:, :cols], d[:, cols:]) if kind != 4 else d
+    # exp and tanh are good to two units, each of a dozen roundings to half a one; where 1 + tanh cancels (or sigmoid's exponential dominates) the error is absolute, against |u| or |u + 1| times a few
+    rel, size = 32 * 2.0 ** -24, (d[:, cols:].abs() + 1) * (d[:, :cols].abs() + 1) if kind in (1, 3) else 0.0
+    err = rel * v.abs() + rel * size
+    s = orc.scales(v)
+    es = torch.stack([e.amax(-1) / 448 for e in err.split(128, -1)], -1) + 2.0 ** -23 * s
+    assert ((scale[:, :-1].double() - s).abs() <= es).all()
+    f = orc.per_column(scale[:, :-1], cols)
+    assert orc.between(q[:, :cols].contiguous().view(F8).double(), v / f, err / f + 3 * 2.0 ** -24 * (v / f).abs()).all()
+    assert (q[:, cols:] == 0x55).all() and (scale[:, -1] == 3.0).all()
+
+
+def test_blocks_of_zeros_of_tiny_and_of_huge_values():
+    v = torch.zeros(4, 384, device="cuda")
+    v[1] = 1e-44; v[1, 130] = 1e-39
+    v[2] = 3e38
+    v[3, :128] = 2.0 ** -125; v[3, 128:256] = -448.0; v[3, 256] = 1.0
+    q, scale = codes(4, 384), torch.zeros(4, 3, device="cuda")
+    glu(4, 0, v, 384, q, scale); sync()
+    got = q.view(F8).double()
+    assert torch.isfinite(got).all() and torch.isfinite(scale).all()
+    assert (scale[0] == orc.TINY).all() and (got[0] == 0).all() and (scale[1] == orc.TINY).all()
+    # (1e-44 is 8.5e-7 of the smallest scale, below half of the smallest e4m3, 2^-10; 1e-39 is 0.085 of it, a number that e4m3 holds to half a step)
+    assert (got[1] == orc.e4m3(v[1].double() / orc.TINY)).all() and float(got[1, 130]) > 0.08
+    back = got * orc.per_column(scale, 384)
+    assert ((back - v.double()).abs() <= 2.0 ** -4 * v.double().abs() + 2.0 ** -10 * orc.per_column(scale, 384)).all()
+    assert (got[3, 128:256] == -448).all()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_what_is_no_number_stays_none(bad, dtype):
+    """a block with an infinity or a NaN stands for NaN; its neighbours and the other rows are as they were; a product carries it to its row alone"""
+    g = gen(5)
+    v = torch.randn(3, 400, generator=g, device="cuda").to(TYPES[dtype])
+    q0, s0 = codes(3, 400), torch.zeros(3, 4, device="cuda")
+    glu(4, dtype, v, 400, q0, s0)
+    v[1, 200] = bad
+    q, s = codes(3, 400), torch.zeros(3, 4, device="cuda")
+    glu(4, dtype, v, 400, q, s)
+    back = q.view(F8).double() * orc.per_column(s, 400)
+    assert back[1, 128:256].isnan().all()
+    back[1, 128:256], old = 0.0, q0.view(F8).double() * orc.per_column(s0, 400)
+    old[1, 128:256] = 0.0
+    assert torch.equal(back, old)
+    w, sw = orc.matrix(40, 400, 3)
+    c = torch.zeros(3, 40, device="cuda")
+    linear(w, sw, q, s, 3, 400, None, 0, 0, c); sync()
+    assert c[1].isnan().all() and torch.isfinite(c[0]).all() and torch.isfinite(c[2]).all()
+    x = torch.randn(2, 256, generator=g, device="cuda").to(TYPES[dtype])
+    x[0, 3] = bad
+    q, s = codes(2, 256), torch.zeros(2, 2, device="cuda")
+    norm(dtype, x, None, None, 1.0, 1e-5, 256, None, q, s); sync()
+    back = q.view(F8).double() * orc.per_column(s, 256)
+    assert not torch.isfinite(back[0, 3]) and torch.isfinite(back[1]).all()
+
+
+# ---------------------------------------------------------------- products
+def check_product(c, want, bound, dtype, extra=0.0, loose=0.0):
+    tol = bound + (want.abs() + bound) * HALF_STEP[dtype] + (2.0 ** -25 if dtype == 1 else 0.0) + extra
+    off = (c.double() - want).abs()
+    assert (off <= tol).all(), float((off / tol).max())
+    # all of them together: what the 8-bit instructions cut off is 2^-13 of the largest of eight products at most, of either sign; the sum of n such sums is off by 2^-13 of its typical size at most
+    assert float(off.norm()) <= (HALF_STEP[dtype] + 2.0 ** -13 + loose) * float(want.norm()) + 1e-30
+
+
+LINEAR_SHAPES = [(1, 16, 16), (1, 100, 144), (1, 4096, 512), (2, 33, 2064), (3, 257, 128), (4, 48, 4000), (5, 300, 1408), (8, 128, 256), (9, 1000, 272), (16, 64, 640), (17, 130, 912), (24, 704, 2064),
+                 (33, 96, 384), (47, 1040, 1024), (64, 513, 144), (65, 257, 768), (100, 640, 400), (127, 384, 2048), (128, 128, 128), (129, 129, 144), (200, 1000, 1040), (256, 512, 256), (257, 300, 512),
+                 (300, 2050, 1408), (511, 1300, 656), (1030, 264, 1024), (40, 4096, 4096), (1500, 1552, 384)]
+
+
+@pytest.mark.parametrize("tokens,rows,cols", LINEAR_SHAPES)
+def test_product(tokens, rows, cols):
+    a0, sa0 = orc.quantised(tokens, cols, tokens + cols)
+    w, sw = orc.matrix(rows, cols, rows)
+    g = gen(tokens * rows)
+    a = torch.full((tokens, cols + 32), 0x7F, dtype=torch.uint8, device="cuda")          # NaN behind the rows
+    a[:, :cols] = a0.view(torch.uint8)
+    sa = padded(sa0, sa0.shape[1] + 2, math.nan)
+    bounds = {wide: orc.product(a0, sa0, w, sw, wide) for wide in (True, False)}
+    bias = torch.randn(rows, generator=g, device="cuda").to(torch.bfloat16)
+    for dtype, accumulate, biased, ws in ((0, 0, True, True), (0, 1, False, False), (1, 0, False, True), (2, 0, True, False), (2, 1, True, True)):
+        c0 = torch.randn(tokens, rows, generator=g, device="cuda").to(TYPES[dtype])
+        c = padded(c0, rows + 5, 6.0)
+        linear(w, sw, a, sa, tokens, cols, bias if biased else None, accumulate, dtype, c, room(rows, cols, tokens) if ws else None); sync()
+        want, bound = bounds[dtype == 0]
+        full = want + (bias.double() if biased else 0.0) + (c0.double() if accumulate else 0.0)
+        check_product(c[:, :rows], full, bound + 2 * 2.0 ** -24 * (want.abs() + 8), dtype)
+        assert (c[:, rows:] == 6.0).all()
+
+
+def test_product_is_the_same_every_time_and_whatever_is_beside_a_row():
+    a, sa = orc.quantised(200, 1040, 1)
+    w, sw = orc.matrix(520, 1040, 2)
+    out = []
+    for ws in (True, True, False):
+        c = torch.zeros(200, 520, device="cuda")
+        linear(w, sw, a, sa, 200, 1040, None, 0, 0, c, room(520, 1040, 200) if ws else None); sync()
+        out.append(c)
+    assert torch.equal(out[0], out[1])
+    assert (out[0] - out[2]).abs().max() <= 1e-5 * out[0].abs().max()
+    a2, sa2 = a.clone(), sa.clone()
+    a2.view(torch.uint8)[100:] = 0x7F; sa2[100:] = math.nan
+    c = torch.zeros(200, 520, device="cuda")
+    linear(w, sw, a2, sa2, 200, 1040, None, 0, 0, c, room(520, 1040, 200)); sync()
+    assert torch.equal(c[:100], out[0][:100]) and c[100:].isnan().all()
+
+
+def test_product_with_offsets_past_32_bits():
+    rows, cols, tokens = 66000, 65536 + 16, 3          # 4.3 GB of values; an output stride that takes rows apart by 2^31 values
+    w = torch.zeros(rows, cols, dtype=torch.uint8, device="cuda").view(F8)
+    sw = torch.ones(orc.blocks(rows), orc.blocks(cols), device="cuda")
+    a, sa = orc.quantised(tokens, cols, 1)
+    last, sl = orc.matrix(16, cols, 2)
+    w.view(torch.uint8)[-16:] = last.view(torch.uint8)
+    sw[-1] = sl[0]
+    c = torch.full((tokens, (1 << 31) + 8), 1.0, dtype=torch.float16, device="cuda")
+    linear(w, sw, a, sa, tokens, cols, None, 0, 1, c); sync()
+    want, bound = orc.product(a, sa, last, sl, False)
+    check_product(c[:, rows - 16:rows], want, bound, 1)
+    assert (c[:, :rows - 16] == 0).all() and (c[:, rows:rows + 100] == 1).all() and (c[:, -100:] == 1).all()
+
+
+def test_many_rows_with_offsets_past_32_bits():
+    rows, cols, tokens = 300, 128, 520
+    a, sa = orc.quantised(tokens, cols, 1)
+    w, sw = orc.matrix(rows, cols, 2)
+    ldc = (1 << 23) + 8          # the last rows lie 2^32 values on
+    c = torch.full((tokens, ldc), 1.0, dtype=torch.bfloat16, device="cuda")
+    linear(w, sw, a, sa, tokens, cols, None, 0, 2, c, room(rows, cols, tokens)); sync()
+    want, bound = orc.product(a, sa, w, sw, False)
+    check_product(c[:, :rows], want, bound, 2)
+    assert (c[:, rows:rows + 64] == 1).all()
+
+
+# ---------------------------------------------------------------- the router
+ROUTES = [(1, 8, 4, 2, True, 64, 6), (1, 1, 1, 2, False, 7, 3), (0, 4, 2, 2, True, 32, 8), (0, 12, 5, 1, False, 180, 10), (1, 8, 8, 1, True, 256, 8), (1, 64, 3, 2, False, 1024, 16), (0, 2, 1, 2, True, 2, 1),
+          (1, 5, 3, 2, True, 5, 3), (0, 1, 1, 1, True, 1000, 64), (1, 16, 4, 2, True, 48, 12), (0, 3, 1, 2, False, 6, 2), (1, 12, 12, 2, True, 384, 9)]
+
+
+@pytest.mark.parametrize("score,groups,kept,best,renorm,n,top", ROUTES)
+@pytest.mark.parametrize("corrected", [True, False])
+def test_router(score, groups, kept, best, renorm, n, top, corrected):
+    g = torch.Generator().manual_seed(n + top)
+    z = 2 * torch.randn(70, n, generator=g)
+    z[10:25] = (2 * z[10:25]).round() / 2          # ties
+    z[11] = 0.25
+    z[26:40][torch.rand(14, n, generator=g) < 0.6] = -math.inf
+    z[40] = -math.inf
+    z[41:45][torch.rand(4, n, generator=g) < 0.3] = math.nan
+    z[45] = math.nan
+    z[46] = 90.0; z[47] = -90.0; z[48] *= 30
+    corr = 0.1 * torch.randn(n, generator=g) if corrected else None
+    if corrected:
+        corr[n // 2] = -3.0
+    eps, scale = (1e-20, 2.5) if renorm else (0.0, 1.0)
+    idx, wgt = route(score, groups, kept, best, renorm, eps, scale, z, corr, top, ld=n + 3); sync()
+    want_i, want_w = orc.route(score, groups, kept, best, renorm, eps, scale, z, corr, top)
+    assert torch.equal(idx.cpu(), want_i)
+    # 64-bit throughout; one rounding to 32 bits (and what lies below the smallest 32-bit number)
+    assert ((wgt.cpu().double() - want_w).abs() <= 2.0 ** -24 * (1 + 1e-6) * want_w.abs() + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 5, 64, 1000, 5003])
+def test_router_over_many_rows(rows):
+    z, corr = torch.randn(rows, 64, generator=torch.Generator().manual_seed(rows)), 0.05 * torch.randn(64, generator=torch.Generator().manual_seed(1))
+    idx, wgt = route(1, 8, 3, 2, True, 1e-20, 2.5, z, corr, 6); sync()
+    pick = torch.arange(rows) if rows <= 64 else torch.randperm(rows, generator=torch.Generator().manual_seed(2))[:64]
+    want_i, want_w = orc.route(1, 8, 3, 2, True, 1e-20, 2.5, z[pick], corr, 6)
+    assert torch.equal(idx.cpu()[pick], want_i) and ((wgt.cpu()[pick].double() - want_w).abs() <= 2.0 ** -24 * (1 + 1e-6) * want_w).all()
+    assert (idx >= 0).all() and (idx.sort(-1).values.diff(dim=-1) > 0).all()          # (no expert twice)
+
+
+# ---------------------------------------------------------------- experts
+# An activation that is off by d moves to the next e4m3 value (a step away, up to 2^-3 of it) with probability d / step: over many, sqrt(step d) of their size; d is 2^-13 at most (above): 2^-8.
+FLIPS = 2.0 ** -8
+
+
+def expert_case(rows, width, ff, E, top, seed, dropped=0.0, one=False):
+    g = gen(seed)
+    a, sa = orc.quantised(rows, width, seed)
+    gu, sgu = orc.matrix(ff, width, seed + 2, count=2 * E, std=2.0 * width ** -0.5)
+    down, sdown = orc.matrix(width, ff, seed + 3, count=E, std=ff ** -0.5)
+    idx = torch.rand(rows, E, generator=g, device="cuda").argsort(-1)[:, :top].to(torch.int32).contiguous()
+    if one:
+        idx[:] = E - 1          # every choice the same expert: the same pair of a row more than once, one long list
+    idx[torch.rand(rows, top, generator=g, device="cuda") < dropped] = -1
+    wgt = torch.randn(rows, top, generator=g, device="cuda")
+    return a, sa, gu.view(E, 2, ff, width), sgu.view(E, 2, orc.blocks(ff), orc.blocks(width)), down, sdown, idx, wgt
+
+
+EXPERT_SHAPES = [(1, 64, 48, 4, 2, 0), (1, 2048, 1408, 16, 6, 0), (2, 144, 128, 3, 3, 1), (3, 272, 400, 8, 1, 3), (5, 1024, 704, 32, 4, 0), (9, 400, 272, 5, 2, 1), (17, 512, 256, 4, 4, 2), (40, 256, 144, 60, 8, 0),
+                 (53, 1040, 336, 8, 2, 3), (130, 384, 640, 3, 1, 0), (301, 528, 208, 6, 3, 1), (700, 256, 384, 2, 2, 0), (1100, 128, 128, 64, 5, 0)]
+
+
+@pytest.mark.parametrize("rows,width,ff,E,top,kind", EXPERT_SHAPES)
+@pytest.mark.parametrize("dropped,one", [(0.0, False), (0.3, False), (0.0, True)])
+def test_experts(rows, width, ff, E, top, kind, dropped, one):
+    a0, sa0, gu, sgu, down, sdown, idx, wgt = expert_case(rows, width, ff, E, top, rows + width + ff, dropped, one)
+    bounds = {wide: orc.experts(kind, a0, sa0, gu, sgu, down, sdown, idx, wgt, wide) for wide in (True, False)}
+    a = torch.full((rows, width + 16), 0x7F, dtype=torch.uint8, device="cuda")
+    a[:, :width] = a0.view(torch.uint8)
+    sa = padded(sa0, sa0.shape[1] + 1, math.nan)
+    for dtype, accumulate in ((0, 0), (0, 1), (1, 0), (2, 1)):
+        y0 = torch.randn(rows, width, generator=gen(1), device="cuda").to(TYPES[dtype])
+        y = padded(y0, width + 3, 4.0)
+        experts(kind, a, sa, width, gu, sgu, down, sdown, idx, wgt, dtype, y, accumulate); sync()
+        want, bound = bounds[dtype == 0]
+        check_product(y[:, :width], want + (y0.double() if accumulate else 0.0), bound, dtype, extra=2.0 ** -24 * (want.abs() + 8), loose=FLIPS)
+        assert (y[:, width:] == 4.0).all()
+
+
+def test_experts_of_rows_that_chose_none_and_of_indices_outside():
+    a, sa, gu, sgu, down, sdown, idx, wgt = expert_case(20, 128, 64, 4, 2, 3)
+    idx[3] = -1; idx[4, 0] = 4; idx[5, 1] = 1 << 30; idx[6] = -(1 << 31); wgt[3:7] = math.nan
+    kept = idx.clone()
+    kept[(idx < 0) | (idx >= 4)] = -1
+    wgt[4, 1] = wgt[5, 0] = 0.5
+    for rows in (20, 7, 1):
+        y = torch.full((rows, 128), 7.0, device="cuda")
+        experts(0, a[:rows].contiguous(), sa[:rows].contiguous(), 128, gu, sgu, down, sdown, idx[:rows].contiguous(), wgt[:rows].contiguous(), 0, y, 0); sync()
+        want, bound = orc.experts(0, a[:rows], sa[:rows], gu, sgu, down, sdown, kept[:rows], wgt[:rows].nan_to_num(0.0), True)
+        check_product(y, want, bound, 0, loose=FLIPS)
+        if rows > 3:
+            assert (y[3] == 0).all()
+    none = torch.full((20, 2), -1, dtype=torch.int32, device="cuda")
+    for accumulate, left in ((0, 0.0), (1, 7.0)):
+        y = torch.full((20, 128), 7.0, device="cuda")
+        experts(0, a, sa, 128, gu, sgu, down, sdown, none, wgt, 0, y, accumulate); sync()
+        assert (y == left).all()
+
+
+@pytest.mark.parametrize("rows", [1, 6, 70, 600])
+def test_a_row_of_the_experts_is_the_same_every_time_and_keeps_its_neighbours_out(rows):
+    a, sa, gu, sgu, down, sdown, idx, wgt = expert_case(rows, 256, 192, 6, 3, 11)
+    out = []
+    for _ in range(3):
+        y = torch.zeros(rows, 256, device="cuda")
+        experts(0, a, sa, 256, gu, sgu, down, sdown, idx, wgt, 0, y, 0); sync()
+        out.append(y)
+    assert torch.equal(out[0], out[1]) and torch.equal(out[0], out[2])
+    if rows > 1:
+        sa2 = sa.clone()
+        sa2[rows - 1] = math.nan
+        y = torch.zeros(rows, 256, device="cuda")
+        experts(0, a, sa2, 256, gu, sgu, down, sdown, idx, wgt, 0, y, 0); sync()
+        assert torch.equal(y[:-1], out[0][:-1]) and y[-1].isnan().all()
+
+
+def test_experts_with_offsets_past_32_bits():
+    rows, width, ff, E = 5, 8192, 8192, 34          # 2.2 GB of down, 4.6 GB of gate and up: the last experts lie past 2^32 bytes
+    a, sa = orc.quantised(rows, width, 1)
+    gu, down = torch.zeros(E, 2, ff, width, dtype=torch.uint8, device="cuda"), torch.zeros(E, width, ff, dtype=torch.uint8, device="cuda")
+    sgu, sdown = torch.ones(E, 2, 64, 64, device="cuda"), torch.ones(E, 64, 64, device="cuda")
+    for e in (32, 33):
+        q, s = orc.matrix(ff, width, e, count=2, std=width ** -0.5)
+        gu[e], sgu[e] = q.view(torch.uint8), s
+        q, s = orc.matrix(width, ff, e + 9, std=ff ** -0.5)
+        down[e], sdown[e] = q.view(torch.uint8), s
+    idx = torch.tensor([[33, 32], [32, 0], [33, -1], [5, 33], [31, 30]], dtype=torch.int32, device="cuda")
+    wgt = torch.full((5, 2), 0.5, device="cuda")
+    want, bound = orc.experts(0, a, sa, gu.view(F8), sgu, down.view(F8), sdown, idx, wgt, True)
+    y = torch.zeros(rows, width, device="cuda")
+    experts(0, a, sa, width, gu.view(F8), sgu, down.view(F8), sdown, idx, wgt, 0, y, 0); sync()
+    check_product(y, want, bound, 0, loose=FLIPS)
+    assert (y[4] == 0).all()
+
+
+# ---------------------------------------------------------------- together
+class Block:
+    """a feed-forward as a serving step runs it: residual and norm, router, experts and a shared expert, all added into the residual"""
+
+    def __init__(self, rows, width=512, ff=256, E=16, top=4, seed=3):
+        g = gen(seed)
+        self.rows, self.width, self.ff, self.E, self.top = rows, width, ff, E, top
+        self.x0, self.m = 2 * torch.randn(rows, width, generator=g, device="cuda"), torch.randn(rows, width, generator=g, device="cuda")
+        self.w = (1 + 0.1 * torch.randn(width, generator=g, device="cuda")).to(torch.bfloat16)
+        self.router = (0.1 * torch.randn(E, width, generator=g, device="cuda")).to(torch.bfloat16)
+        self.corr = 0.02 * torch.randn(E, generator=g, device="cuda")
+        _, _, self.gu, self.sgu, self.down, self.sdown, _, _ = expert_case(1, width, ff, E, top, seed)
+        self.shared_up, self.s_shared_up = orc.matrix(2 * ff, width, 7, std=2.0 * width ** -0.5)
+        self.shared_down, self.s_shared_down = orc.matrix(width, ff, 8, std=ff ** -0.5)
+        self.x, self.h, self.q, self.s = torch.empty_like(self.x0), torch.empty_like(self.x0), codes(rows, width), torch.empty(rows, orc.blocks(width), device="cuda")
+        self.z, self.idx, self.wgt = torch.empty(rows, E, device="cuda"), torch.empty(rows, top, dtype=torch.int32, device="cuda"), torch.empty(rows, top, device="cuda")
+        self.act, self.aq, self.asc = torch.empty(rows, 2 * ff, device="cuda"), codes(rows, ff), torch.empty(rows, orc.blocks(ff), device="cuda")
+        L = capi()
+        self.ws = torch.empty(max(L.ifa_moe_experts_fp8_workspace_bytes(rows, top, width, ff, E), L.ifa_linear_fp8_workspace_bytes(2 * ff, width, rows), L.ifa_linear_fp8_workspace_bytes(width, ff, rows), 16),
+                              dtype=torch.uint8, device="cuda")
+
+    def step(self):
+        L, s, r, W = capi(), here(), self.rows, self.width
+        at = lambda t: t.data_ptr()  # noqa: E731
+        self.x.copy_(self.x0)
+        ia.check(L.ifa_norm_add_fp8(0, at(self.x), W, r, W, at(self.m), W, at(self.w), 0.0, 1e-5, at(self.h), W, at(self.q), W, at(self.s), self.s.shape[1], s))
+        ia.check(L.ifa_linear_bf16w(at(self.router), self.E, W, at(self.h), W, r, None, None, 1.0, 0, 1, at(self.z), self.E, 0, 0, s))
+        ia.check(L.ifa_moe_route_groups_f32(1, 4, 2, 2, 1, 1e-20, 1.5, at(self.z), self.E, r, self.E, self.top, at(self.corr), at(self.idx), at(self.wgt), s))
+        ia.check(L.ifa_moe_experts_fp8(0, 0.0, at(self.q), W, at(self.s), self.s.shape[1], r, W, self.ff, self.E, self.top, at(self.gu), at(self.sgu), at(self.down), at(self.sdown), at(self.idx),
+                                       at(self.wgt), at(self.ws), self.ws.numel(), 0, at(self.x), W, 1, s))
+        ia.check(L.ifa_linear_fp8(at(self.shared_up), at(self.s_shared_up), 2 * self.ff, W, at(self.q), W, at(self.s), self.s.shape[1], r, None, 0, 0, at(self.act), 2 * self.ff, at(self.ws),
+                                  self.ws.numel(), s))
+        ia.check(L.ifa_glu_fp8(0, 0.0, 0, at(self.act), 2 * self.ff, r, self.ff, at(self.aq), self.ff, at(self.asc), self.asc.shape[1], s))
+        ia.check(L.ifa_linear_fp8(at(self.shared_down), at(self.s_shared_down), W, self.ff, at(self.aq), self.ff, at(self.asc), self.asc.shape[1], r, None, 1, 0, at(self.x), W, at(self.ws),
+                                  self.ws.numel(), s))
+
+    def check(self):
+        """against 64 bits, from the quantised rows on (each quantisation is checked by itself above)"""
+        x = (self.x0 + self.m).double()
+        v = x / torch.sqrt(x.square().mean(-1, keepdim=True) + 1e-5) * self.w.double()
+        check_quantised(self.q, self.s, v, NORM_ERR)
+        z = v @ self.router.double().t()
+        assert (self.z.double() - z).abs().max() < 1e-4
+        idx, wgt = orc.route(1, 4, 2, 2, True, 1e-20, 1.5, self.z.cpu(), self.corr.cpu(), self.top)
+        assert torch.equal(self.idx.cpu(), idx) and (self.wgt.cpu().double() - wgt).abs().max() < 1e-6
+        q = self.q.view(F8)
+        y, bound = orc.experts(0, q, self.s, self.gu, self.sgu, self.down, self.sdown, self.idx, self.wgt, True, 0.0)
+        up, ub = orc.product(q, self.s, self.shared_up, self.s_shared_up, True)
+        assert ((self.act.double() - up).abs() <= ub).all()
+        d, db = orc.product(self.aq.view(F8), self.asc, self.shared_down, self.s_shared_down, True)
+        check_product(self.x, x + y + d, bound + db, 0, extra=4 * 2.0 ** -24 * (x.abs() + y.abs() + d.abs()), loose=FLIPS)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 20, 150, 1030])
+def test_a_feed_forward_as_it_is_used(rows):
+    b = Block(rows)
+    b.step(); sync()
+    b.check()
+
+
+@pytest.mark.parametrize("rows", [1, 20, 150])
+def test_captured_and_replayed_beside_eager_work(rows):
+    """two captured steps that share a workspace, replayed in turn with eager work and synchronisations between, on new inputs"""
+    b, other = Block(rows, seed=3), Block(rows, seed=8)
+    other.ws = b.ws
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        b.step(); other.step()
+    torch.cuda.current_stream().wait_stream(side)
+    sync()
+    graphs = []
+    for block in (b, other):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            block.step()
+        graphs.append(graph)
+    for turn in range(4):
+        for block, graph in zip((b, other), graphs):
+            block.x0.copy_(torch.randn(block.x0.shape, generator=gen(turn), device="cuda"))
+            block.x.fill_(math.nan)
+            graph.replay()
+            if turn % 2:
+                sync()
+        sync()
+        got = [t.clone() for t in (b.x, other.x, b.idx, other.idx)]
+        b.step(); sync(); other.step(); sync()
+        assert all(torch.equal(u, v) for u, v in zip(got, (b.x, other.x, b.idx, other.idx)))
+        b.check()
+
+
+def test_two_streams_at_once():
+    blocks, streams = [Block(40, seed=s) for s in (1, 2)], [torch.cuda.Stream() for _ in range(2)]
+    sync()
+    for _ in range(3):
+        for block, stream in zip(blocks, streams):
+            with torch.cuda.stream(stream):
+                block.step()
+    sync()
+    for block in blocks:
+        block.check()
