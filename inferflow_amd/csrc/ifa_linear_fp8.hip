@@ -4,6 +4,7 @@
 // never meets another block's before it has its scale.  16-bit outputs take the 8-bit instructions, 32-bit outputs exact halves (ifa_fp8.h).
 #include "ifa_host.h"
 #include "ifa_fp8_stream.h"
+#include "ifa_fp8_tile.h"
 
 using namespace ifa8;
 
@@ -15,12 +16,12 @@ template <int DT> __device__ __forceinline__ void store_out(typename Elem<DT>::t
     *c = (typename Elem<DT>::type)v;
 }
 
-template <int DT, int TILES>
-__global__ void __launch_bounds__(64 * STREAM_WAVES) k_linear_fp8_stream(const uint8_t *__restrict__ w, const float *__restrict__ sw, int rows, int cols, const uint8_t *__restrict__ a, size_t lda,
+template <int DT, int TILES, int WAVES, int DEPTH>
+__global__ void __launch_bounds__(64 * WAVES) k_linear_fp8_stream(const uint8_t *__restrict__ w, const float *__restrict__ sw, int rows, int cols, const uint8_t *__restrict__ a, size_t lda,
                                                                         const float *__restrict__ sa, size_t lds, int tokens, const bf16_t *__restrict__ bias, int accumulate,
                                                                         typename Elem<DT>::type *__restrict__ c, size_t ldc)
 {
-    __shared__ f32x4 red[(STREAM_WAVES - 1) * TILES * 64];
+    __shared__ f32x4 red[(WAVES - 1) * TILES * 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n0 = blockIdx.x * 16, t0 = blockIdx.y * 16 * TILES;
     const uint8_t *wr[1] = {w + (size_t)min(n0 + (lane & 15), rows - 1) * cols};
     const float *swr[1] = {sw + (size_t)(n0 / BLOCK) * blocks_of(cols)};
@@ -34,8 +35,8 @@ __global__ void __launch_bounds__(64 * STREAM_WAVES) k_linear_fp8_stream(const u
         sar[j] = sa + t * lds;
         acc[0][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    stream_blocks<DT == IFA_F32, 1, TILES>(wr, swr, ar, sar, cols, wave, STREAM_WAVES, acc);
-    join_waves<1, TILES>(acc, red);
+    stream_blocks<DT == IFA_F32, DEPTH, 1, TILES>(wr, swr, ar, sar, cols, wave, WAVES, acc);
+    join_waves<WAVES, 1, TILES>(acc, red);
     if (wave > 0) return;
 #pragma unroll
     for (int j = 0; j < TILES; j++) {
@@ -49,21 +50,89 @@ __global__ void __launch_bounds__(64 * STREAM_WAVES) k_linear_fp8_stream(const u
     }
 }
 
-template <int DT>
-int linear(const void *w, const void *sw, size_t rows, size_t cols, const void *a, size_t lda, const void *sa, size_t lds, size_t tokens, const void *bias, int accumulate, void *c, size_t ldc,
-           void *ws, size_t ws_bytes, hipStream_t s)
+template <int DT, class T, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN, 2) k_linear_fp8_tile(const uint8_t *__restrict__ w, const float *__restrict__ sw, int rows, int cols, const uint8_t *__restrict__ a, size_t lda,
+                                                                     const float *__restrict__ sa, size_t lds, int tokens, const bf16_t *__restrict__ bias, int accumulate,
+                                                                     typename Elem<DT>::type *__restrict__ c, size_t ldc, int tiles_t, int tiles_n, int whole)
 {
-    typedef typename Elem<DT>::type T;
-#define IFA_STREAM(TILES)                                                                                                                                                  \
-    hipLaunchKernelGGL((k_linear_fp8_stream<DT, TILES>), dim3((unsigned)((rows + 15) / 16), (unsigned)((tokens + 16 * TILES - 1) / (16 * TILES))), dim3(64 * STREAM_WAVES), 0, s, \
-                       (const uint8_t *)w, (const float *)sw, (int)rows, (int)cols, (const uint8_t *)a, lda, (const float *)sa, lds, (int)tokens, (const bf16_t *)bias, accumulate,  \
-                       (T *)c, ldc)
-    if (tokens <= 16) IFA_STREAM(1);
-    else if (tokens <= 32) IFA_STREAM(2);
-    else IFA_STREAM(4);
-#undef IFA_STREAM
+    constexpr int BM = T::TM * 16 * WM, BN = T::TN * 16 * WN, BAND = 8;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % WM, wn = wave / WM;
+    // bands of eight activation tiles, the tiles of a band fastest
+    const int at = xcd_place(blockIdx.x, tiles_t * tiles_n), band = at / (BAND * tiles_n), within = at % (BAND * tiles_n), band_t = min(BAND, tiles_t - band * BAND);
+    const int t0 = (band * BAND + within % band_t) * BN, n0 = within / band_t * BM;
+    f32x4 acc[T::TM][T::TN];
+#pragma unroll
+    for (int j = 0; j < T::TN; j++)
+#pragma unroll
+        for (int m = 0; m < T::TM; m++) acc[m][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int nw = n0 + wm * (BM / WM), tw = t0 + wn * (BN / WN);          // the wave's first rows
+    const float *swr = sw + (size_t)(min(nw, rows - 1) / BLOCK) * blocks_of(cols);
+    tile_sums<DT == IFA_F32, true, T>(
+        smem, cols, w + (size_t)n0 * cols, [&](int r) { return (uint32_t)min(r, rows - 1 - n0) * (uint32_t)cols; }, [&](int r) { return a + (size_t)min(t0 + r, tokens - 1) * lda; },
+        [&](int m) { return wm * (BM / WM) + 16 * m; }, [&](int, int b) { return swr[b]; }, sa + (size_t)min(tw + lane, tokens - 1) * lds, wn * (BN / WN), acc);
+    constexpr int N = VEC<DT>;
+    tile_out<T, N>(smem, acc, [&](int t, int n, float *v) {
+        t += tw; n += nw;
+        if (t >= tokens || n >= rows) return;
+        typename Elem<DT>::type *d = c + (size_t)t * ldc + n;
+        if (whole) {
+            if (bias) {
+#pragma unroll
+                for (int e = 0; e < N; e++) v[e] += ifa32::bf2f(bias[n + e]);
+            }
+            if (accumulate) {
+                float old[N];
+                unpack<DT>(*reinterpret_cast<const u32x4 *>(d), old);
+#pragma unroll
+                for (int e = 0; e < N; e++) v[e] += old[e];
+            }
+            *reinterpret_cast<u32x4 *>(d) = pack<DT>(v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                if (n + e < rows) store_out<DT>(d + e, v[e] + (bias ? ifa32::bf2f(bias[n + e]) : 0.0f), accumulate);
+        }
+    });
+}
+
+struct Product {
+    const uint8_t *w; const float *sw; size_t rows, cols; const uint8_t *a; size_t lda; const float *sa; size_t lds, tokens; const bf16_t *bias; int accumulate; void *c; size_t ldc;
+};
+
+template <int DT, int TILES, int WAVES, int DEPTH>
+int launch_stream(const Product &P, hipStream_t s)
+{
+    hipLaunchKernelGGL((k_linear_fp8_stream<DT, TILES, WAVES, DEPTH>), dim3((unsigned)((P.rows + 15) / 16), (unsigned)((P.tokens + 16 * TILES - 1) / (16 * TILES))), dim3(64 * WAVES), 0, s, P.w, P.sw,
+                       (int)P.rows, (int)P.cols, P.a, P.lda, P.sa, P.lds, (int)P.tokens, P.bias, P.accumulate, (typename Elem<DT>::type *)P.c, P.ldc);
     IFA_LAUNCH_CHECK();
     return IFA_OK;
+}
+
+template <int DT, int BM, int BN, int WM, int WN>
+int launch_tile(const Product &P, hipStream_t s)
+{
+    typedef Tile<BM, BN, WM, WN> T;
+    const auto fn = k_linear_fp8_tile<DT, T, WM, WN>;
+    const size_t tt = (P.tokens + BN - 1) / BN, tn = (P.rows + BM - 1) / BM;
+    if (P.cols > (1u << 22)) return launch_stream<DT, 4, 8, 1>(P, s);          // (a tile's offsets have 32 bits)
+    IFA_REQUIRE(tt * tn < (1u << 31), "ifa_linear_fp8: too many tiles");
+    const bool whole = P.rows % VEC<DT> == 0 && P.ldc % VEC<DT> == 0 && ((uintptr_t)P.c & 15) == 0;          // 16 bytes of output at a time
+    if (T::SMEM > 64 * 1024) IFA_HIP_CHECK(hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, T::SMEM));
+    hipLaunchKernelGGL(fn, dim3((unsigned)(tt * tn)), dim3(64 * WM * WN), T::SMEM, s, P.w, P.sw, (int)P.rows, (int)P.cols, P.a, P.lda, P.sa, P.lds, (int)P.tokens, P.bias, P.accumulate,
+                       (typename Elem<DT>::type *)P.c, P.ldc, (int)tt, (int)tn, (int)whole);
+    IFA_LAUNCH_CHECK();
+    return IFA_OK;
+}
+
+template <int DT>
+int linear(const Product &P, hipStream_t s)
+{
+    if (P.tokens <= 16) return launch_stream<DT, 1, 8, 1>(P, s);
+    if (P.tokens <= 32) return launch_stream<DT, 2, 8, 1>(P, s);
+    if (P.tokens <= 64) return launch_stream<DT, 4, 8, 1>(P, s);
+    if (DT != IFA_F32 && P.tokens > 256 && P.rows > 512) return launch_tile<DT, 256, 256, 2, 4>(P, s);
+    return launch_tile<DT, 128, 128, 2, 2>(P, s);
 }
 
 } // namespace
@@ -82,8 +151,9 @@ int ifa_linear_fp8(const void *w_e4m3, const void *w_scale_f32, size_t rows, siz
     IFA_REQUIRE(lda >= cols && lda % 16 == 0 && lds >= blocks_of(cols) && ldc >= rows, "ifa_linear_fp8: row strides");
     IFA_REQUIRE((((uintptr_t)w_e4m3 | (uintptr_t)a_e4m3 | (uintptr_t)ws) & 15) == 0 && (((uintptr_t)w_scale_f32 | (uintptr_t)a_scale_f32) & 3) == 0 && ((uintptr_t)bias_bf16 & 1) == 0
                     && (uintptr_t)c % elem_bytes(c_dtype) == 0, "ifa_linear_fp8: misaligned pointer");
-    auto f = c_dtype == IFA_F32 ? linear<IFA_F32> : c_dtype == IFA_F16 ? linear<IFA_F16> : linear<IFA_BF16>;
-    return f(w_e4m3, w_scale_f32, rows, cols, a_e4m3, lda, a_scale_f32, lds, tokens, bias_bf16, accumulate, c, ldc, ws, ws_bytes, ifa_s(stream));
+    const Product P = {(const uint8_t *)w_e4m3, (const float *)w_scale_f32, rows, cols, (const uint8_t *)a_e4m3, lda, (const float *)a_scale_f32, lds, tokens, (const bf16_t *)bias_bf16, accumulate, c,
+                       ldc};
+    return c_dtype == IFA_F32 ? linear<IFA_F32>(P, ifa_s(stream)) : c_dtype == IFA_F16 ? linear<IFA_F16>(P, ifa_s(stream)) : linear<IFA_BF16>(P, ifa_s(stream));
 }
 
 } // extern "C"

@@ -5,194 +5,558 @@
 #include <algorithm>
 #include "ifa_host.h"
 #include "ifa_fp8_stream.h"
+#include "ifa_fp8_tile.h"
 
 using namespace ifa8;
 
 namespace {
 
-// One wave per row.  Scores and choices in 64 bits: two experts whose choices differ by less than a 32-bit rounding are told apart as the formula does.
-__global__ void __launch_bounds__(64) k_moe_route_groups(const float *__restrict__ logits, size_t ld, int n_all, int top, int score_kind, int groups, int kept, int best_of, int renorm,
-                                                         float renorm_eps, float wgt_scale, const float *__restrict__ corr, int *__restrict__ idx, float *__restrict__ wgt)
+// ---- the router.  One wave per row, four rows a workgroup; lane l holds the choices of experts l, l + 64, ...  Scores and choices in 64 bits: two experts whose choices differ by less than a 32-bit
+// rounding are told apart as the formula does.  Bound by instructions (64-bit exponentials and quotients, a maximum over the wave for each expert taken), not by the logits' bytes; so the
+// choices are kept as integers that order like them, and the maximum is one of their upper halves (a comparison of 32 bits a step between lanes) unless two are equal there.
+constexpr int ROUTE_ROWS = 4;
+
+__device__ __forceinline__ uint64_t order_of(double v)          // orders like v; 0: no choice
 {
-    extern __shared__ double sc[];          // [n_all] scores, [n_all] choices
-    double *ch = sc + n_all;
-    const int lane = threadIdx.x, each = n_all / groups;
-    const size_t t = blockIdx.x;
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return v > -INFINITY ? ((u >> 63) ? ~u : u | 0x8000000000000000ull) : 0ull;          // (false for a NaN)
+}
+__device__ __forceinline__ double value_of(uint64_t o) { return __builtin_bit_cast(double, (o >> 63) ? o & 0x7FFFFFFFFFFFFFFFull : ~o); }
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v)
+{
+    v = group_max<16>(v);
+    v = dpp_max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false));          // rows 1 and 3: the row in front of them too
+    v = dpp_max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false));          // rows 2 and 3: the half in front of them
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane)
+{
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+template <int CTRL> __device__ __forceinline__ uint64_t dpp_u64(uint64_t v)
+{
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_mov_dpp((int)(v >> 32), CTRL, 0xF, 0xF, true) << 32) | (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
+}
+
+template <int PER>
+__global__ void __launch_bounds__(64 * ROUTE_ROWS) k_moe_route_groups(const float *__restrict__ logits, size_t ld, int rows, int n_all, int top, int score_kind, int groups, int kept, int best_of,
+                                                                      int renorm, float renorm_eps, float wgt_scale, const float *__restrict__ corr, int *__restrict__ idx, float *__restrict__ wgt)
+{
+    __shared__ uint64_t grp[ROUTE_ROWS][64 * PER];          // a row's choices, for its groups
+    __shared__ double sc[ROUTE_ROWS][64 * PER];              // and its scores
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, each = n_all / groups;
+    const size_t t = (size_t)blockIdx.x * ROUTE_ROWS + wave;
+    if (t >= (size_t)rows) return;
     const float *z = logits + t * ld;
-    auto logit = [&](int e) { const float v = z[e]; return v == v ? v : -INFINITY; };
-    double mx = 0.0, all = 1.0;
+    float v[PER], c[PER];
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        const int e = lane + 64 * j;
+        const float x = e < n_all ? z[e] : -INFINITY;
+        v[j] = x == x ? x : -INFINITY;
+        c[j] = corr && e < n_all ? corr[e] : 0.0f;
+    }
+    double s[PER];
     if (score_kind == 0) {
         float m = -INFINITY;
-        for (int e = lane; e < n_all; e += 64) m = fmaxf(m, logit(e));
-        mx = (double)ifa32::wave_max(m);
-        all = 0.0;
-        for (int e = lane; e < n_all; e += 64) all += exp((double)logit(e) - mx);
+#pragma unroll
+        for (int j = 0; j < PER; j++) m = fmaxf(m, v[j]);
+        const double mx = (double)ifa32::wave_max(m);
+        double all = 0.0;
+#pragma unroll
+        for (int j = 0; j < PER; j++) { s[j] = exp((double)v[j] - mx); all += lane + 64 * j < n_all ? s[j] : 0.0; }
         for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o, 64);
+        all = 1.0 / all;
+#pragma unroll
+        for (int j = 0; j < PER; j++) s[j] *= all;
+    } else {
+#pragma unroll
+        for (int j = 0; j < PER; j++) s[j] = 1.0 / (1.0 + exp(-(double)v[j]));
     }
-    for (int e = lane; e < n_all; e += 64) {
-        const float v = logit(e);
-        const double s = score_kind == 0 ? exp((double)v - mx) / all : 1.0 / (1.0 + exp(-(double)v));
-        const double c = s + (corr ? (double)corr[e] : 0.0);
-        sc[e] = s;
-        ch[e] = v > -INFINITY && c == c ? c : -INFINITY;
+    uint32_t hi[PER], lo[PER];
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        const uint64_t o = v[j] > -INFINITY ? order_of(s[j] + (double)c[j]) : 0ull;
+        hi[j] = (uint32_t)(o >> 32); lo[j] = (uint32_t)o;
+        sc[wave][lane + 64 * j] = s[j];
+        if (groups > 1) grp[wave][lane + 64 * j] = o;
     }
-    __syncthreads();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");          // (a wave reads what it has written itself)
     if (groups > 1) {
-        double value = -INFINITY;          // lane g: of group g
-        if (lane < groups) {
-            double b0 = -INFINITY, b1 = -INFINITY;
-            for (int e = lane * each; e < (lane + 1) * each; e++) { const double c = ch[e]; if (c > b0) { b1 = b0; b0 = c; } else if (c > b1) b1 = c; }
-            value = b0 + (best_of > 1 && b1 > -INFINITY ? b1 : 0.0);
-        }
+        // a group's best two by `per` neighbouring lanes, each over its part of the group
+        const int per = 64 >> (32 - __builtin_clz(groups - 1)), g = lane / per;
+        uint64_t b0 = 0, b1 = 0;
+        if (g < groups)
+            for (int e = g * each + lane % per; e < (g + 1) * each; e += per) { const uint64_t o = grp[wave][e]; if (o > b0) { b1 = b0; b0 = o; } else if (o > b1) b1 = o; }
+        auto merge = [&](uint64_t p0, uint64_t p1) { b1 = max(min(b0, p0), max(b1, p1)); b0 = max(b0, p0); };
+        if (per > 1) merge(dpp_u64<0xB1>(b0), dpp_u64<0xB1>(b1));
+        if (per > 2) merge(dpp_u64<0x4E>(b0), dpp_u64<0x4E>(b1));
+        if (per > 4) merge(dpp_u64<0x141>(b0), dpp_u64<0x141>(b1));
+        if (per > 8) merge(dpp_u64<0x128>(b0), dpp_u64<0x128>(b1));
+        if (per > 16) merge(__shfl_xor(b0, 16, 64), __shfl_xor(b1, 16, 64));
+        const double value = b0 == 0 ? -INFINITY : value_of(b0) + (best_of > 1 && b1 != 0 ? value_of(b1) : 0.0);
         int better = 0;
-        for (int g = 0; g < groups; g++) { const double o = __shfl(value, g, 64); better += o > value || (o == value && g < lane); }
-        if (lane < groups && better >= kept) for (int e = lane * each; e < (lane + 1) * each; e++) ch[e] = -INFINITY;
-        __syncthreads();
+        for (int o = 0; o < groups; o++) {
+            const double other = __builtin_bit_cast(double, read_lane(__builtin_bit_cast(uint64_t, value), o * per));
+            better += other > value || (other == value && o < g);
+        }
+        const uint64_t stays = __ballot(better < kept);
+#pragma unroll
+        for (int j = 0; j < PER; j++)
+            if (!((stays >> (min((lane + 64 * j) / each, groups - 1) * per)) & 1)) hi[j] = 0;
     }
-    double sum = 0.0, mine = 0.0;
     int at = -1;
     for (int k = 0; k < top; k++) {
-        double best = -INFINITY; int bi = n_all;
-        for (int e = lane; e < n_all; e += 64) { const double v = ch[e]; if (v > best) { best = v; bi = e; } }
-        for (int o = 32; o > 0; o >>= 1) {
-            const double ov = __shfl_xor(best, o, 64); const int oi = __shfl_xor(bi, o, 64);
-            if (ov > best || (ov == best && oi < bi)) { best = ov; bi = oi; }
+        uint32_t m = hi[0];
+#pragma unroll
+        for (int j = 1; j < PER; j++) m = dpp_max(m, hi[j]);
+        m = wave_max_u32(m);
+        if (m == 0) break;          // (a choice's upper half is not 0)
+        uint64_t who[PER];
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < PER; j++) { who[j] = __ballot(hi[j] == m); n += __popcll(who[j]); }
+        if (n > 1) {          // the same upper half: by the lower ones
+            uint32_t l = 0;
+#pragma unroll
+            for (int j = 0; j < PER; j++) if (hi[j] == m) l = dpp_max(l, lo[j]);
+            l = wave_max_u32(l);
+#pragma unroll
+            for (int j = 0; j < PER; j++) who[j] = __ballot(hi[j] == m && lo[j] == l);
         }
-        const bool found = bi < n_all;
-        const double s = found ? sc[bi] : 0.0;
-        sum += s;
-        if (lane == k) { at = found ? bi : -1; mine = s; }
-        if (found && lane == 0) ch[bi] = -INFINITY;
-        __syncthreads();
+        int e = -1;
+#pragma unroll
+        for (int j = PER - 1; j >= 0; j--) if (who[j]) e = 64 * j + __builtin_ctzll(who[j]);          // (the lowest index of equals)
+#pragma unroll
+        for (int j = 0; j < PER; j++) if (e == lane + 64 * j) hi[j] = 0;
+        if (lane == k) at = e;
+    }
+    double mine = at >= 0 ? sc[wave][at] : 0.0;
+    if (renorm) {
+        double sum = mine;
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        const double den = sum + (double)renorm_eps;
+        mine = den > 0.0 ? mine / den : 0.0;
     }
     if (lane < top) {
-        if (renorm) { const double den = sum + (double)renorm_eps; mine = den > 0.0 ? mine / den : 0.0; }
         idx[t * top + lane] = at;
         wgt[t * top + lane] = (float)(mine * (double)wgt_scale);
     }
 }
 
-// ONE workgroup: the pairs (row, choice) sorted by expert.  place_row[at] = the row of the pair at sorted place `at`, pair_at[p] = the place of pair p (-1: none), tiles = {expert, first
-// place, places} of at most `tile` places of one expert.  A pair's place within its expert's range is a matter of order alone: no value depends on it.
-__global__ void __launch_bounds__(1024) k_moe_fp8_sort(const int *__restrict__ idx, int pairs, int experts, int top, int tile, int *__restrict__ place_row, int *__restrict__ pair_at,
-                                                       int *__restrict__ tiles, int *__restrict__ n_tiles)
+// ---- one to a few rows, two launches: every (row, choice) pair streams its expert's matrices.
+// act[p][n] = act(Gate_e a) (Up_e a) of pair p; grid (16 columns each, pairs), the blocks of columns shared out to the waves
+constexpr int PAIR_WAVES = 8;
+__global__ void __launch_bounds__(64 * PAIR_WAVES) k_moe_fp8_up_pairs(const uint8_t *__restrict__ gu, const float *__restrict__ sgu, int width, int ff, int experts, int top,
+                                                                      const uint8_t *__restrict__ a, size_t lda, const float *__restrict__ sa, size_t lds, const int *__restrict__ idx, int kind,
+                                                                      float limit, float *__restrict__ act)
 {
-    extern __shared__ int cnt[];          // [experts] counts, then cursors; [experts] first places
-    int *off = cnt + experts;
-    for (int e = threadIdx.x; e < experts; e += blockDim.x) cnt[e] = 0;
-    __syncthreads();
-    for (int p = threadIdx.x; p < pairs; p += blockDim.x) { const int e = idx[p]; if (e >= 0 && e < experts) atomicAdd(&cnt[e], 1); }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        int o = 0, nt = 0;
-        for (int e = 0; e < experts; e++) {
-            off[e] = o;
-            for (int r = 0; r < cnt[e]; r += tile) { tiles[3 * nt] = e; tiles[3 * nt + 1] = o + r; tiles[3 * nt + 2] = min(tile, cnt[e] - r); nt++; }
-            o += cnt[e];
-            cnt[e] = 0;
-        }
-        *n_tiles = nt;
-    }
-    __syncthreads();
-    for (int p = threadIdx.x; p < pairs; p += blockDim.x) {
-        const int e = idx[p];
-        if (e < 0 || e >= experts) { pair_at[p] = -1; continue; }
-        const int at = off[e] + atomicAdd(&cnt[e], 1);
-        place_row[at] = p / top; pair_at[p] = at;
+    __shared__ f32x4 red[(PAIR_WAVES - 1) * 2 * 64];
+    const int p = blockIdx.y, e = idx[p];
+    if (e < 0 || e >= experts) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n0 = blockIdx.x * 16;
+    const size_t n = n0 + (lane & 15), wb = blocks_of(width), fb = blocks_of(ff), t = p / top;          // (ff in whole 16s)
+    const uint8_t *wr[2] = {gu + ((size_t)e * 2 * ff + n) * width, gu + ((size_t)(e * 2 + 1) * ff + n) * width};
+    const float *swr[2] = {sgu + ((size_t)e * 2 * fb + n0 / BLOCK) * wb, sgu + ((size_t)(e * 2 + 1) * fb + n0 / BLOCK) * wb};
+    const uint8_t *ar[1] = {a + t * lda};
+    const float *sar[1] = {sa + t * lds};
+    f32x4 acc[2][1];
+    acc[0][0] = acc[1][0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    stream_blocks<false, 1, 2, 1>(wr, swr, ar, sar, width, wave, PAIR_WAVES, acc);
+    join_waves<PAIR_WAVES, 2, 1>(acc, red);
+    if (wave > 0 || (lane & 15)) return;          // (the sixteen activation rows of the products are one and the same)
+    f32x4 v;
+#pragma unroll
+    for (int r = 0; r < 4; r++) v[r] = ifa32::glu_of(kind, limit, acc[0][0][r], acc[1][0][r]);
+    *reinterpret_cast<f32x4 *>(act + (size_t)p * ff + n0 + 4 * (lane >> 4)) = v;
+}
+
+// 32-bit activations of pairs into e4m3 in LDS: item it = block it % fb of pair pair(it / fb) (-1: zeros); [items] blocks of 128 bytes and their scales.  Half a wave an item.
+template <class Pair> __device__ __forceinline__ void quantise_items(const float *__restrict__ act, int ff, int fb, int items, Pair pair, char *q, float *sc)
+{
+    for (int it = threadIdx.x >> 5; it < items; it += blockDim.x >> 5) {
+        const int k = it / fb, b = it - k * fb, p = pair(k), c = b * BLOCK + 4 * (threadIdx.x & 31);
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (p >= 0 && c < ff) unpack<IFA_F32>(*reinterpret_cast<const u32x4 *>(act + (size_t)p * ff + c), v);
+        uint32_t most = 0u;
+#pragma unroll
+        for (int r = 0; r < 4; r++) most = dpp_max(most, abs_bits(v[r]));
+        most = group_max<32>(most);
+        const float s = scale_of(most);
+        *reinterpret_cast<uint32_t *>(q + it * BLOCK + 4 * (threadIdx.x & 31)) = quantise4(v, 1.0f / s);
+        if ((threadIdx.x & 31) == 0) sc[it] = p >= 0 ? s : 0.0f;
     }
 }
 
-// act[at][n] = act(Gate_e a) (Up_e a) for the places of a tile; grid (16 columns each, tiles)
-template <int TILES>
-__global__ void __launch_bounds__(64 * STREAM_WAVES) k_moe_fp8_up(const uint8_t *__restrict__ gu, const float *__restrict__ sgu, int width, int ff, const uint8_t *__restrict__ a, size_t lda,
-                                                                 const float *__restrict__ sa, size_t lds, const int *__restrict__ place_row, const int *__restrict__ tiles,
-                                                                 const int *__restrict__ n_tiles, int kind, float limit, float *__restrict__ act)
+// y[t][c] (+)= sum_k wgt Down_e q(act[t, k]); grid (8 columns each, rows).  Of the sixteen matrix rows of a product eight are of one choice's expert and eight, the same columns, of another's; their
+// activations are its columns 0 and 1 (with sixteen columns of one expert 2048 columns are 128 workgroups, half of the compute units: 14 us).  A workgroup quantises its row's activations into LDS
+// itself (again in every workgroup: a launch of its own would take longer), its first weights on their way meanwhile.
+template <int DT, int AHEAD>
+__global__ void __launch_bounds__(64 * PAIR_WAVES) k_moe_fp8_down_pairs(const uint8_t *__restrict__ down, const float *__restrict__ sdown, int width, int ff, int experts, int top,
+                                                                        const float *__restrict__ act, const int *__restrict__ idx, const float *__restrict__ wgt,
+                                                                        typename Elem<DT>::type *__restrict__ y, size_t ldy, int accumulate)
 {
-    if ((int)blockIdx.y >= *n_tiles) return;
-    __shared__ f32x4 red[(STREAM_WAVES - 1) * 2 * TILES * 64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n0 = blockIdx.x * 16, e = tiles[3 * blockIdx.y], at0 = tiles[3 * blockIdx.y + 1], n_at = tiles[3 * blockIdx.y + 2];
-    const size_t n = min(n0 + (lane & 15), ff - 1), wb = blocks_of(width), fb = blocks_of(ff);
-    const uint8_t *wr[2] = {gu + ((size_t)e * 2 * ff + n) * width, gu + ((size_t)(e * 2 + 1) * ff + n) * width};
-    const float *swr[2] = {sgu + ((size_t)e * 2 * fb + n0 / BLOCK) * wb, sgu + ((size_t)(e * 2 + 1) * fb + n0 / BLOCK) * wb};
+    constexpr bool WIDE = DT == IFA_F32;
+    extern __shared__ __attribute__((aligned(16))) char smem[];          // [2 pairs of choices * fb] blocks of 128 bytes, their scales
+    __shared__ f32x4 red[(PAIR_WAVES - 1) * 64];
+    __shared__ int expert[64];
+    __shared__ float weight[64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n0 = blockIdx.x * 8, fb = (int)blocks_of(ff), both = (top + 1) / 2, items = both * fb, p0 = blockIdx.y * top;
+    const size_t wb = blocks_of(width);
+    float *const sc = reinterpret_cast<float *>(smem + (size_t)2 * items * BLOCK);
+    if (threadIdx.x < 2 * both) {
+        const int e = (int)threadIdx.x < top ? idx[p0 + threadIdx.x] : -1;
+        expert[threadIdx.x] = e >= 0 && e < experts ? e : -1;
+        weight[threadIdx.x] = (int)threadIdx.x < top ? wgt[p0 + threadIdx.x] : 0.0f;
+    }
+    __syncthreads();
+    // item: block item % fb of choices 2 k and 2 k + 1, k = item / fb.  A lane's matrix row: column n0 + lane % 8 of choice 2 k + (lane / 8) % 2; its results': choice 2 k + lane / 32
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    struct Group { u32x4 w[AHEAD][2]; float f[AHEAD]; };
+    auto ask = [&](Group &G, int first) {
+#pragma unroll
+        for (int d = 0; d < AHEAD; d++) {
+            const int it = first + d * PAIR_WAVES, k = it < items ? it / fb : 0, b = it - k * fb, c = b * BLOCK + 16 * g;
+            const int e = it < items ? expert[2 * k + ((lane >> 3) & 1)] : -1, er = it < items ? expert[2 * k + (lane >> 5)] : -1;
+            const uint8_t *w = down + ((size_t)max(e, 0) * width + n0 + (lane & 7)) * ff + c;
+            G.w[d][0] = e >= 0 && c < ff ? *reinterpret_cast<const u32x4 *>(w) : zero;
+            G.w[d][1] = e >= 0 && c + 64 < ff ? *reinterpret_cast<const u32x4 *>(w + 64) : zero;
+            G.f[d] = er >= 0 ? sdown[((size_t)er * wb + n0 / BLOCK) * fb + b] * weight[2 * k + (lane >> 5)] : 0.0f;
+        }
+    };
+    Group G[2];
+    ask(G[0], wave);
+    quantise_items(act, ff, fb, 2 * items, [&](int k) { return expert[k] >= 0 ? p0 + k : -1; }, smem, sc);
+    __syncthreads();
+    f32x4 acc[1][1];
+    acc[0][0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    auto go = [&](const Group &G, int first) {
+#pragma unroll
+        for (int d = 0; d < AHEAD; d++) {
+            const int it = first + d * PAIR_WAVES;
+            if (it >= items) break;
+            const int k = it / fb, b = it - k * fb;
+            Operand<WIDE> av, wv;
+            const char *q = smem + ((2 * k + (lane & 1)) * fb + b) * BLOCK + 16 * g;
+            av.set(*reinterpret_cast<const u32x4 *>(q), *reinterpret_cast<const u32x4 *>(q + 64));
+            wv.set(G.w[d][0], G.w[d][1]);
+            const f32x4 x = mfma128(wv, av);
+            const float s = sc[(2 * k + (lane >> 5)) * fb + b];
+            if (expert[2 * k + (lane >> 5)] >= 0)          // (a choice that is none: whatever its weight is)
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[0][0][r] = fmaf(x[r], G.f[d] * s, acc[0][0][r]);
+        }
+    };
+    for (int it = wave; it < items; it += 2 * AHEAD * PAIR_WAVES) {
+        ask(G[1], it + AHEAD * PAIR_WAVES);
+        go(G[0], it);
+        ask(G[0], it + 2 * AHEAD * PAIR_WAVES);
+        go(G[1], it + AHEAD * PAIR_WAVES);
+    }
+    join_waves<PAIR_WAVES, 1, 1>(acc, red);
+    if (wave > 0) return;
+    // lane 0 / 16: columns 0 .. 3 / 4 .. 7 of the first choices; lane 33 / 49: of the second ones
+#pragma unroll
+    for (int r = 0; r < 4; r++) acc[0][0][r] += __shfl(acc[0][0][r], (lane + 33) & 63, 64);
+    if (lane != 0 && lane != 16) return;
+    typename Elem<DT>::type *d = y + (size_t)blockIdx.y * ldy + n0 + 4 * g;
+#pragma unroll
+    for (int r = 0; r < 4; r++) d[r] = (typename Elem<DT>::type)(accumulate ? (float)d[r] + acc[0][0][r] : acc[0][0][r]);
+}
+
+// ---- a few rows for each expert, three launches: a workgroup finds the pairs of its expert itself, in their order, and streams its part of the expert's matrices past all of them.
+constexpr int LIST_MAX = 2048;          // pairs of a step
+constexpr int LIST_WAVES = 4;
+// pairs p with idx[p] == e in list[0 .. n); every thread gets n
+template <int WAVES> __device__ __forceinline__ int list_pairs(const int *__restrict__ idx, int pairs, int e, uint16_t *list, int *counts)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int n = 0;
+    for (int p0 = 0; p0 < pairs; p0 += 64 * WAVES) {
+        const int p = p0 + threadIdx.x;
+        const bool mine = p < pairs && idx[p] == e;
+        const uint64_t who = __ballot(mine);
+        if (lane == 0) counts[wave] = __popcll(who);
+        __syncthreads();
+        int at = n;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) { if (w < wave) at += counts[w]; n += counts[w]; }
+        if (mine) list[at + __popcll(who & ((1ull << lane) - 1))] = (uint16_t)p;
+        __syncthreads();
+    }
+    return n;
+}
+
+// act[p] of the expert's pairs; grid (16 columns each, experts), the blocks of columns shared out to the waves.  (A workgroup of 128 columns, a wave 16 of them, could quantise them too: few workgroups,
+// 22.6 + 3.4 -> 32.5 us for 53 rows of four of 32 experts, 2048 x 704.)
+template <int TILES>
+__device__ __forceinline__ void up_list(const uint16_t *list, int n, const uint8_t *const (&wr)[2], const float *const (&swr)[2], int n0, int width, int ff, int top, const uint8_t *a, size_t lda,
+                                        const float *sa, size_t lds, int kind, float limit, float *act, f32x4 *red)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15;
     const uint8_t *ar[TILES];
     const float *sar[TILES];
     f32x4 acc[2][TILES];
 #pragma unroll
     for (int j = 0; j < TILES; j++) {
-        const size_t t = place_row[at0 + min(16 * j + (lane & 15), n_at - 1)];
-        ar[j] = a + t * lda;
-        sar[j] = sa + t * lds;
+        const size_t t = list[min(16 * j + i, n - 1)] / top;
+        ar[j] = a + t * lda; sar[j] = sa + t * lds;
         acc[0][j] = acc[1][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    stream_blocks<false, 2, TILES>(wr, swr, ar, sar, width, wave, STREAM_WAVES, acc);
-    join_waves<2, TILES>(acc, red);
-    if (wave > 0) return;
+    stream_blocks<false, 1, 2, TILES>(wr, swr, ar, sar, width, wave, LIST_WAVES, acc);
+    join_waves<LIST_WAVES, 2, TILES>(acc, red);
+    if (wave == 0) {
 #pragma unroll
-    for (int j = 0; j < TILES; j++) {
-        const int at = 16 * j + (lane & 15);
-        if (at >= n_at) continue;
+        for (int j = 0; j < TILES; j++) {
+            if (16 * j + i >= n) continue;
+            f32x4 v;
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int c = n0 + 4 * (lane >> 4) + r;
-            if (c < ff) act[(size_t)(at0 + at) * ff + c] = ifa32::glu_of(kind, limit, acc[0][j][r], acc[1][j][r]);
+            for (int r = 0; r < 4; r++) v[r] = ifa32::glu_of(kind, limit, acc[0][j][r], acc[1][j][r]);
+            *reinterpret_cast<f32x4 *>(act + (size_t)list[16 * j + i] * ff + n0 + 4 * (lane >> 4)) = v;
         }
     }
+    __syncthreads();          // (`red` is read)
 }
-
-// rows of 32-bit activations in places that the tiles hold, into e4m3: a workgroup of two rows of lanes a block
-__global__ void __launch_bounds__(256) k_moe_fp8_quantise(const float *__restrict__ act, int ff, const int *__restrict__ tiles, const int *__restrict__ n_tiles, uint8_t *__restrict__ q, float *__restrict__ s)
+__global__ void __launch_bounds__(64 * LIST_WAVES) k_moe_fp8_up_list(const uint8_t *__restrict__ gu, const float *__restrict__ sgu, int width, int ff, int pairs, int top,
+                                                                     const uint8_t *__restrict__ a, size_t lda, const float *__restrict__ sa, size_t lds, const int *__restrict__ idx, int kind,
+                                                                     float limit, float *__restrict__ act)
 {
-    if ((int)blockIdx.y >= *n_tiles) return;
-    const int at0 = tiles[3 * blockIdx.y + 1], n_at = tiles[3 * blockIdx.y + 2], fb = (int)blocks_of(ff);
-    for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < n_at * fb; i += gridDim.x * 8) {
-        const size_t at = at0 + i / fb;
-        const int b = i % fb, c = b * BLOCK + 4 * (threadIdx.x & 31);
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (c < ff) unpack<IFA_F32>(*reinterpret_cast<const u32x4 *>(act + at * ff + c), v);
-        uint32_t most = 0u;
-#pragma unroll
-        for (int e = 0; e < 4; e++) most = dpp_max(most, abs_bits(v[e]));
-        most = group_max<32>(most);
-        const float sc = scale_of(most);
-        if (c < ff) *reinterpret_cast<uint32_t *>(q + at * ff + c) = quantise4(v, 1.0f / sc);
-        if ((threadIdx.x & 31) == 0) s[at * fb + b] = sc;
+    __shared__ uint16_t list[LIST_MAX];
+    __shared__ int counts[LIST_WAVES];
+    __shared__ f32x4 red[(LIST_WAVES - 1) * 2 * 2 * 64];
+    const int e = blockIdx.y, n = list_pairs<LIST_WAVES>(idx, pairs, e, list, counts), lane = threadIdx.x & 63, n0 = blockIdx.x * 16;          // (ff in whole 16s)
+    const size_t r0 = n0 + (lane & 15), wb = blocks_of(width), fb = blocks_of(ff);
+    const uint8_t *wr[2] = {gu + ((size_t)e * 2 * ff + r0) * width, gu + ((size_t)(e * 2 + 1) * ff + r0) * width};
+    const float *swr[2] = {sgu + ((size_t)e * 2 * fb + n0 / BLOCK) * wb, sgu + ((size_t)(e * 2 + 1) * fb + n0 / BLOCK) * wb};
+    for (int at = 0; at < n; at += 32) {
+        if (n - at <= 16) up_list<1>(list + at, n - at, wr, swr, n0, width, ff, top, a, lda, sa, lds, kind, limit, act, red);
+        else up_list<2>(list + at, n - at, wr, swr, n0, width, ff, top, a, lda, sa, lds, kind, limit, act, red);
     }
 }
 
-// out[at][c] = Down_e q[at]; grid (16 columns each, tiles)
-template <bool WIDE, int TILES>
-__global__ void __launch_bounds__(64 * STREAM_WAVES) k_moe_fp8_down(const uint8_t *__restrict__ down, const float *__restrict__ sdown, int width, int ff, const uint8_t *__restrict__ q,
-                                                                   const float *__restrict__ s, const int *__restrict__ tiles, const int *__restrict__ n_tiles, float *__restrict__ out)
+// out[p] of the expert's pairs, 16 at a time; grid (128 columns, experts), a wave 16 columns and all their blocks.  The workgroup quantises the pairs' activations into LDS itself.
+constexpr int DOWN_WAVES = 8;
+constexpr int DOWN_FF = 4096;          // at most: 16 rows in LDS
+template <bool WIDE>
+__global__ void __launch_bounds__(64 * DOWN_WAVES) k_moe_fp8_down_list(const uint8_t *__restrict__ down, const float *__restrict__ sdown, int width, int ff, int pairs, const int *__restrict__ idx,
+                                                                       const float *__restrict__ act, float *__restrict__ out)
 {
-    if ((int)blockIdx.y >= *n_tiles) return;
-    __shared__ f32x4 red[(STREAM_WAVES - 1) * TILES * 64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n0 = blockIdx.x * 16, e = tiles[3 * blockIdx.y], at0 = tiles[3 * blockIdx.y + 1], n_at = tiles[3 * blockIdx.y + 2];
+    constexpr int AHEAD = 3;
+    extern __shared__ __attribute__((aligned(16))) char smem[];          // [16 * fb] blocks of 128 bytes, their scales
+    __shared__ uint16_t list[LIST_MAX];
+    __shared__ int counts[DOWN_WAVES];
+    const int e = blockIdx.y, lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15, n0 = blockIdx.x * 16 * DOWN_WAVES + 16 * (threadIdx.x >> 6), fb = (int)blocks_of(ff);
+    float *const sc = reinterpret_cast<float *>(smem + (size_t)16 * fb * BLOCK);
+    const bool live = n0 < width;          // (width in whole 16s)
+    const uint8_t *const w = down + ((size_t)e * width + (live ? n0 : 0) + i) * ff;
+    const float *const sw = sdown + ((size_t)e * blocks_of(width) + (live ? n0 : 0) / BLOCK) * fb;
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    struct Group { u32x4 w[AHEAD][2]; float f[AHEAD]; };
+    auto ask = [&](Group &G, int b0) {
+#pragma unroll
+        for (int d = 0; d < AHEAD; d++) {
+            const int b = min(b0 + d, fb - 1), c = b * BLOCK + 16 * g;
+            G.w[d][0] = c < ff ? *reinterpret_cast<const u32x4 *>(w + c) : zero;
+            G.w[d][1] = c + 64 < ff ? *reinterpret_cast<const u32x4 *>(w + c + 64) : zero;
+            G.f[d] = sw[b];
+        }
+    };
+    const int n = list_pairs<DOWN_WAVES>(idx, pairs, e, list, counts);
+    for (int at = 0; at < n; at += 16) {
+        const int here = min(n - at, 16);
+        Group G[2];
+        ask(G[0], 0);
+        if (at > 0) __syncthreads();          // (the rows before are read)
+        quantise_items(act, ff, fb, here * fb, [&](int k) { return (int)list[at + k]; }, smem, sc);
+        __syncthreads();
+        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        const int row = min(i, here - 1) * fb;
+        auto go = [&](const Group &G, int b0) {
+#pragma unroll
+            for (int d = 0; d < AHEAD; d++) {
+                const int b = b0 + d;
+                if (b >= fb) break;
+                Operand<WIDE> av, wv;
+                const char *q = smem + (row + b) * BLOCK + 16 * g;
+                av.set(*reinterpret_cast<const u32x4 *>(q), *reinterpret_cast<const u32x4 *>(q + 64));
+                wv.set(G.w[d][0], G.w[d][1]);
+                const f32x4 x = mfma128(wv, av);
+                const float f = G.f[d] * sc[row + b];
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[r] = fmaf(x[r], f, acc[r]);
+            }
+        };
+        for (int b = 0; b < fb; b += 2 * AHEAD) {
+            ask(G[1], b + AHEAD);
+            go(G[0], b);
+            ask(G[0], b + 2 * AHEAD);
+            go(G[1], b + AHEAD);
+        }
+        if (live && i < here) *reinterpret_cast<f32x4 *>(out + (size_t)list[at + i] * width + n0 + 4 * g) = acc;
+    }
+}
+
+// ---- many rows: the pairs sorted by expert.  k_moe_fp8_count leaves, for each block of `per` pairs, how many of them chose each expert; k_moe_fp8_place adds these counts up and gives the pairs
+// their places: place_row[at] = the row of the pair at sorted place `at`, pair_at[p] = the place of pair p (-1: none), tiles = {expert, first place, places} of at most PLACES places of one
+// expert, *n_tiles.  (A workgroup alone took 31 us for 18000 pairs.)  A pair's place within its block's part of an expert's range is a matter of order alone: no value depends on it.
+__global__ void __launch_bounds__(1024) k_moe_fp8_count(const int *__restrict__ idx, int pairs, int experts, int per, int *__restrict__ counts)
+{
+    __shared__ int cnt[1024];
+    cnt[threadIdx.x] = 0;
+    __syncthreads();
+    const int p0 = blockIdx.x * per;
+    for (int p = p0 + threadIdx.x; p < min(p0 + per, pairs); p += 1024) { const int e = idx[p]; if (e >= 0 && e < experts) atomicAdd(&cnt[e], 1); }
+    __syncthreads();
+    if ((int)threadIdx.x < experts) counts[blockIdx.x * experts + threadIdx.x] = cnt[threadIdx.x];
+}
+// what stands in front of a thread's value among 1024 threads' values; part: 17 ints
+__device__ __forceinline__ int scan_1024(int v, int *part)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int x = v;
+    for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(x, d, 64); if (lane >= d) x += o; }
+    if (lane == 63) part[wave] = x;
+    __syncthreads();
+    int in_front = 0;
+    for (int w = 0; w < 16; w++) if (w < wave) in_front += part[w];
+    if (threadIdx.x == 1023) part[16] = in_front + x;
+    __syncthreads();
+    return in_front + x - v;
+}
+__global__ void __launch_bounds__(1024) k_moe_fp8_place(const int *__restrict__ idx, int pairs, int experts, int top, int tile, int per, const int *__restrict__ counts, int *__restrict__ place_row,
+                                                        int *__restrict__ pair_at, int *__restrict__ tiles, int *__restrict__ n_tiles)
+{
+    __shared__ int cursor[1024], part[17], part2[17];
+    const int e = threadIdx.x, blocks = gridDim.x;
+    int before = 0, all = 0;
+    if (e < experts)
+        for (int b = 0; b < blocks; b++) { const int c = counts[b * experts + e]; all += c; if (b < (int)blockIdx.x) before += c; }
+    const int first = scan_1024(all, part);
+    cursor[e] = first + before;
+    if (blockIdx.x == 0) {
+        const int nt = (all + tile - 1) / tile, t0 = scan_1024(nt, part2);
+        for (int k = 0; k < nt; k++) { int *t = tiles + 3 * (t0 + k); t[0] = e; t[1] = first + k * tile; t[2] = min(tile, all - k * tile); }
+        if (e == 0) *n_tiles = part2[16];
+    }
+    __syncthreads();
+    const int p0 = blockIdx.x * per;
+    for (int p = p0 + threadIdx.x; p < min(p0 + per, pairs); p += 1024) {
+        const int x = idx[p];
+        if (x < 0 || x >= experts) { pair_at[p] = -1; continue; }
+        const int at = atomicAdd(&cursor[x], 1);
+        place_row[at] = p / top; pair_at[p] = at;
+    }
+}
+
+// Tiles of 64 places of one expert.  A workgroup of four waves, two a compute unit.
+constexpr int PLACES = 64;
+typedef Tile<256, PLACES, 2, 2> MoeTile;
+
+// the tile's place among those that there are (the empty ones behind them are dealt to nobody); tiles of one expert side by side
+__device__ __forceinline__ bool moe_tile(const int *n_tiles, int blocks, int &tile, int &block)
+{
+    const int nt = *n_tiles, all = nt * blocks;
+    if ((int)blockIdx.x >= all) return false;
+    constexpr int BAND = 8;
+    const int at = xcd_place(blockIdx.x, all), band = at / (BAND * blocks), within = at % (BAND * blocks), in_band = min(BAND, nt - band * BAND);
+    tile = band * BAND + within % in_band;
+    block = within / in_band;
+    return true;
+}
+
+// a tile of 128 gate rows and the 128 up rows of the same columns: one block of the activations, which leave it quantised
+__global__ void __launch_bounds__(256, 2) k_moe_fp8_up_tile(const uint8_t *__restrict__ gu, const float *__restrict__ sgu, int width, int ff, const uint8_t *__restrict__ a, size_t lda,
+                                                            const float *__restrict__ sa, size_t lds, const int *__restrict__ place_row, const int *__restrict__ tiles,
+                                                            const int *__restrict__ n_tiles, int kind, float limit, uint8_t *__restrict__ q, float *__restrict__ s)
+{
+    typedef MoeTile T;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1, g = lane >> 4, i = lane & 15, fb = (int)blocks_of(ff);
+    int tile, block;
+    if (!moe_tile(n_tiles, fb, tile, block)) return;
+    const int e = tiles[3 * tile], at0 = tiles[3 * tile + 1], n_at = tiles[3 * tile + 2], n0 = block * BLOCK;
+    f32x4 acc[T::TM][T::TN];
+#pragma unroll
+    for (int m = 0; m < T::TM; m++)
+#pragma unroll
+        for (int j = 0; j < T::TN; j++) acc[m][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const size_t wb = blocks_of(width);
+    const float *sg = sgu + ((size_t)e * 2 * fb + block) * wb, *su = sg + fb * wb;
+    auto row_of = [&](int r) { return (size_t)place_row[at0 + min(r, n_at - 1)]; };
+    tile_sums<false, false, T>(
+        smem, width, gu + (size_t)e * 2 * ff * width, [&](int r) { return (uint32_t)((r < BLOCK ? 0 : ff) + min(n0 + (r & (BLOCK - 1)), ff - 1)) * (uint32_t)width; },
+        [&](int r) { return a + row_of(r) * lda; }, [&](int m) { return (m < 4 ? 0 : BLOCK) + 64 * wm + 16 * (m & 3); }, [&](int m, int b) { return m < 4 ? sg[b] : su[b]; },
+        sa + row_of(32 * wn + (lane & 31)) * lds, 32 * wn, acc);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");          // (the buffers' last block is read)
+    uint32_t *const most = reinterpret_cast<uint32_t *>(smem + PLACES * BLOCK);          // [2 waves][64 places], behind the tile's quantised rows
+    const bool whole = n0 + BLOCK <= ff;
+    uint32_t mine[T::TN];
+#pragma unroll
+    for (int j = 0; j < T::TN; j++) {
+        mine[j] = 0u;
+#pragma unroll
+        for (int m = 0; m < 4; m++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                float v = ifa32::glu_of(kind, limit, acc[m][j][r], acc[m + 4][j][r]);
+                if (!whole && n0 + 64 * wm + 16 * m >= ff) v = 0.0f;          // (ff in whole 16s)
+                acc[m][j][r] = v;
+                mine[j] = dpp_max(mine[j], abs_bits(v));
+            }
+        mine[j] = dpp_max(mine[j], (uint32_t)__shfl_xor((int)mine[j], 16, 64));
+        mine[j] = dpp_max(mine[j], (uint32_t)__shfl_xor((int)mine[j], 32, 64));
+        if (g == 0) most[wm * PLACES + 32 * wn + 16 * j + i] = mine[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < T::TN; j++) {
+        const int at = 32 * wn + 16 * j + i;
+        const float sc = scale_of(dpp_max(most[at], most[PLACES + at])), inv = 1.0f / sc;
+        if (wm == 0 && g == 0 && at < n_at) s[(size_t)(at0 + at) * fb + block] = sc;
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+            const float v[4] = {acc[m][j][0], acc[m][j][1], acc[m][j][2], acc[m][j][3]};
+            *reinterpret_cast<uint32_t *>(smem + at * BLOCK + 16 * ((4 * wm + m) ^ (at & 7)) + 4 * g) = quantise4(v, inv);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = threadIdx.x; k < PLACES * 8; k += 256) {
+        const int at = k >> 3, piece = k & 7;
+        if (at < n_at && n0 + 16 * piece < ff) *reinterpret_cast<u32x4 *>(q + (size_t)(at0 + at) * ff + n0 + 16 * piece) = *reinterpret_cast<const u32x4 *>(smem + at * BLOCK + 16 * (piece ^ (at & 7)));
+    }
+}
+
+template <bool WIDE>
+__global__ void __launch_bounds__(256, 2) k_moe_fp8_down_tile(const uint8_t *__restrict__ down, const float *__restrict__ sdown, int width, int ff, const uint8_t *__restrict__ q,
+                                                              const float *__restrict__ s, const int *__restrict__ tiles, const int *__restrict__ n_tiles, float *__restrict__ out)
+{
+    typedef MoeTile T;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1;
+    int tile, block;
+    if (!moe_tile(n_tiles, (width + 255) / 256, tile, block)) return;
+    const int e = tiles[3 * tile], at0 = tiles[3 * tile + 1], n_at = tiles[3 * tile + 2], n0 = block * 256;
+    f32x4 acc[T::TM][T::TN];
+#pragma unroll
+    for (int m = 0; m < T::TM; m++)
+#pragma unroll
+        for (int j = 0; j < T::TN; j++) acc[m][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const size_t wb = blocks_of(width), fb = blocks_of(ff);
-    const uint8_t *wr[1] = {down + ((size_t)e * width + min(n0 + (lane & 15), width - 1)) * ff};
-    const float *swr[1] = {sdown + ((size_t)e * wb + n0 / BLOCK) * fb};
-    const uint8_t *ar[TILES];
-    const float *sar[TILES];
-    f32x4 acc[1][TILES];
-#pragma unroll
-    for (int j = 0; j < TILES; j++) {
-        const size_t at = at0 + min(16 * j + (lane & 15), n_at - 1);
-        ar[j] = q + at * ff;
-        sar[j] = s + at * fb;
-        acc[0][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    stream_blocks<WIDE, 1, TILES>(wr, swr, ar, sar, ff, wave, STREAM_WAVES, acc);
-    join_waves<1, TILES>(acc, red);
-    if (wave > 0) return;
-#pragma unroll
-    for (int j = 0; j < TILES; j++) {
-        const int at = 16 * j + (lane & 15);
-        if (at < n_at) *reinterpret_cast<f32x4 *>(out + (size_t)(at0 + at) * width + n0 + 4 * (lane >> 4)) = acc[0][j];      // (width % 16 == 0)
-    }
+    const int nw = n0 + 128 * wm;
+    const float *sd = sdown + ((size_t)e * wb + min(nw, width - 1) / BLOCK) * fb;
+    tile_sums<WIDE, true, T>(
+        smem, ff, down + ((size_t)e * width + n0) * ff, [&](int r) { return (uint32_t)min(r, width - 1 - n0) * (uint32_t)ff; },
+        [&](int r) { return q + (size_t)(at0 + min(r, n_at - 1)) * ff; }, [&](int m) { return 128 * wm + 16 * m; }, [&](int, int b) { return sd[b]; },
+        s + (size_t)(at0 + min(32 * wn + (lane & 31), n_at - 1)) * fb, 32 * wn, acc);
+    tile_out<T, 4>(smem, acc, [&](int t, int n, float *v) {
+        if (32 * wn + t < n_at && nw + n < width) *reinterpret_cast<u32x4 *>(out + (size_t)(at0 + 32 * wn + t) * width + nw + n) = pack<IFA_F32>(v);          // (width in whole 16s)
+    });
 }
 
 // y[t][c] (+)= sum over the row's choices, in their order
 template <int DT>
-__global__ void __launch_bounds__(256) k_moe_fp8_join(const float *__restrict__ out, const int *__restrict__ pair_at, const float *__restrict__ wgt, int top, int width, size_t all,
+__global__ void __launch_bounds__(256) k_moe_fp8_join(const float *__restrict__ out, const int *__restrict__ pair_at, const int *__restrict__ idx, int experts, const float *__restrict__ wgt, int top, int width, size_t all,
                                                       typename Elem<DT>::type *__restrict__ y, size_t ldy, int accumulate)
 {
     const size_t id = (size_t)blockIdx.x * 256 + threadIdx.x;
@@ -201,7 +565,7 @@ __global__ void __launch_bounds__(256) k_moe_fp8_join(const float *__restrict__ 
     const int c = (int)(id % (width / 4)) * 4;
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int k = 0; k < top; k++) {
-        const int at = pair_at[t * top + k];
+        const int p = (int)t * top + k, at = pair_at ? pair_at[p] : (idx[p] >= 0 && idx[p] < experts ? p : -1);          // (no places: the pairs' own order)
         if (at < 0) continue;
         const f32x4 v = *reinterpret_cast<const f32x4 *>(out + (size_t)at * width + c);
         const float f = wgt[t * top + k];
@@ -216,17 +580,21 @@ __global__ void __launch_bounds__(256) k_moe_fp8_join(const float *__restrict__ 
 }
 
 // ---- workspace
-size_t up16(size_t n) { return (n + 255) / 256 * 256; }
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 struct Work {
-    size_t lists, tiles, act, q, s, out, bytes;
+    size_t lists, counts, tiles, act, q, s, out, bytes;
+    int per, blocks;          // k_moe_fp8_count's
     Work(size_t rows, size_t top, size_t width, size_t ff, size_t experts)
     {
-        const size_t pairs = rows * top, n_tiles = pairs / 16 + std::min(pairs, experts) + 1;
+        const size_t pairs = rows * top, n_tiles = pairs / PLACES + std::min(pairs, experts) + 1;
+        per = (int)std::max<size_t>(2048, (pairs + 255) / 256);
+        blocks = (int)((pairs + per - 1) / per);
         size_t o = 0;
-        auto take = [&](size_t n) { const size_t at = o; o += up16(n); return at; };
+        auto take = [&](size_t n) { const size_t at = o; o += up256(n); return at; };
         lists = take(8 * pairs + 16);          // place_row, pair_at; the number of tiles
+        counts = take(4 * blocks * experts);
         tiles = take(12 * n_tiles);
-        act = take(4 * pairs * ff);
+        act = take(pairs <= LIST_MAX ? 4 * pairs * ff : 0);
         q = take(pairs * ff);
         s = take(4 * pairs * blocks_of(ff));
         out = take(4 * pairs * width);
@@ -247,8 +615,10 @@ int ifa_moe_route_groups_f32(int score_kind, int groups, int groups_kept, int gr
     IFA_REQUIRE(groups > 0 && groups <= 64 && n_all % groups == 0 && groups_kept > 0 && groups_kept <= groups && (group_best == 1 || group_best == 2),
                 "ifa_moe_route_groups_f32: %d of %d groups by their best %d", groups_kept, groups, group_best);
     IFA_REQUIRE(top > 0 && top <= 64 && top <= groups_kept * (n_all / groups), "ifa_moe_route_groups_f32: %d of %d experts", top, groups_kept * (n_all / groups));
-    hipLaunchKernelGGL(k_moe_route_groups, dim3((unsigned)rows), dim3(64), 2 * (size_t)n_all * sizeof(double), ifa_s(stream), (const float *)logits_f32, ld, n_all, top, score_kind, groups,
-                       groups_kept, group_best, renorm, renorm_eps, wgt_scale, (const float *)correction_f32, idx_dev, (float *)wgt_f32);
+    const int per = (n_all + 63) / 64;
+    const auto fn = per <= 1 ? k_moe_route_groups<1> : per <= 2 ? k_moe_route_groups<2> : per <= 4 ? k_moe_route_groups<4> : per <= 8 ? k_moe_route_groups<8> : k_moe_route_groups<16>;
+    hipLaunchKernelGGL(fn, dim3(ifa_cdiv(rows, ROUTE_ROWS)), dim3(64 * ROUTE_ROWS), 0, ifa_s(stream), (const float *)logits_f32, ld, (int)rows, n_all, top, score_kind, groups, groups_kept,
+                       group_best, renorm, renorm_eps, wgt_scale, (const float *)correction_f32, idx_dev, (float *)wgt_f32);
     IFA_LAUNCH_CHECK();
     return IFA_OK;
 }
@@ -266,7 +636,8 @@ int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t ld
     IFA_REQUIRE(a_e4m3 && a_scale_f32 && gate_up_e4m3 && gate_up_scale_f32 && down_e4m3 && down_scale_f32 && idx_dev && wgt_f32 && ws && y, "ifa_moe_experts_fp8: null pointer");
     if (!elem_known(y_dtype)) return ifa_fail(IFA_ERR_DTYPE, "ifa_moe_experts_fp8: output dtype %d (F32, F16 or BF16)", y_dtype);
     IFA_REQUIRE(glu_kind >= 0 && glu_kind <= 3, "ifa_moe_experts_fp8: activation %d", glu_kind);
-    IFA_REQUIRE(rows > 0 && width > 0 && ff > 0 && width % 16 == 0 && ff % 16 == 0 && experts > 0 && experts <= 1024 && top > 0 && top <= 64 && rows * top <= 1000000 && width <= 65536 && ff <= 65536,
+    IFA_REQUIRE(rows > 0 && width > 0 && ff > 0 && width % 16 == 0 && ff % 16 == 0 && experts > 0 && experts <= 1024 && top > 0 && top <= 64 && rows * top <= 1000000 && width <= 65536 && ff <= 65536
+                    && 2 * (size_t)ff * width < (1ull << 32),
                 "ifa_moe_experts_fp8: %zu rows x %d of %d experts, %d x %d (whole 16s)", rows, top, experts, width, ff);
     IFA_REQUIRE(lda >= (size_t)width && lda % 16 == 0 && lds >= blocks_of(width) && ldy >= (size_t)width, "ifa_moe_experts_fp8: row strides");
     IFA_REQUIRE((((uintptr_t)a_e4m3 | (uintptr_t)gate_up_e4m3 | (uintptr_t)down_e4m3 | (uintptr_t)ws) & 15) == 0 && (((uintptr_t)a_scale_f32 | (uintptr_t)gate_up_scale_f32 | (uintptr_t)down_scale_f32) & 3) == 0
@@ -279,22 +650,44 @@ int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t ld
     float *act = (float *)(base + W.act), *s = (float *)(base + W.s), *out = (float *)(base + W.out);
     uint8_t *q = base + W.q;
     const hipStream_t st = ifa_s(stream);
-    const int tile = pairs / experts >= 32 ? 64 : 16;
-    const unsigned max_tiles = (unsigned)(pairs / tile + std::min(pairs, experts));
-    hipLaunchKernelGGL(k_moe_fp8_sort, dim3(1), dim3(1024), 2 * experts * sizeof(int), st, idx_dev, pairs, experts, top, tile, place_row, pair_at, tiles, n_tiles);
-    const dim3 g_up((unsigned)((ff + 15) / 16), max_tiles), g_down((unsigned)(width / 16), max_tiles), b(64 * STREAM_WAVES);
-    IFA_REQUIRE(max_tiles < 65536, "ifa_moe_experts_fp8: too many rows");
-#define IFA_UP(T) hipLaunchKernelGGL((k_moe_fp8_up<T>), g_up, b, 0, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, (const uint8_t *)a_e4m3, lda, \
-                                     (const float *)a_scale_f32, lds, place_row, tiles, n_tiles, glu_kind, limit, act)
-#define IFA_DOWN(W, T) hipLaunchKernelGGL((k_moe_fp8_down<W, T>), g_down, b, 0, st, (const uint8_t *)down_e4m3, (const float *)down_scale_f32, width, ff, q, s, tiles, n_tiles, out)
-    if (tile == 16) IFA_UP(1); else IFA_UP(4);
-    hipLaunchKernelGGL(k_moe_fp8_quantise, dim3((unsigned)std::min<size_t>((blocks_of(ff) * tile + 7) / 8, 64), max_tiles), dim3(256), 0, st, act, ff, tiles, n_tiles, q, s);
-    if (y_dtype == IFA_F32) { if (tile == 16) IFA_DOWN(true, 1); else IFA_DOWN(true, 4); }
-    else if (tile == 16) IFA_DOWN(false, 1); else IFA_DOWN(false, 4);
-#undef IFA_UP
+    const size_t few_lds = (size_t)2 * ((top + 1) / 2) * blocks_of(ff) * (BLOCK + 4);
+    if (rows <= 4 && few_lds <= 48 * 1024) {
+        hipLaunchKernelGGL(k_moe_fp8_up_pairs, dim3(ff / 16, pairs), dim3(64 * PAIR_WAVES), 0, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, experts, top,
+                           (const uint8_t *)a_e4m3, lda, (const float *)a_scale_f32, lds, idx_dev, glu_kind, limit, act);
+#define IFA_DOWN(DT) hipLaunchKernelGGL((k_moe_fp8_down_pairs<DT, 3>), dim3(width / 8, (unsigned)rows), dim3(64 * PAIR_WAVES), few_lds, st, (const uint8_t *)down_e4m3, (const float *)down_scale_f32, \
+                                        width, ff, experts, top, act, idx_dev, (const float *)wgt_f32, (Elem<DT>::type *)y, ldy, accumulate)
+        if (y_dtype == IFA_F32) IFA_DOWN(IFA_F32); else if (y_dtype == IFA_F16) IFA_DOWN(IFA_F16); else IFA_DOWN(IFA_BF16);
 #undef IFA_DOWN
+        IFA_LAUNCH_CHECK();
+        return IFA_OK;
+    }
+    const bool wide = y_dtype == IFA_F32, many = pairs > LIST_MAX || pairs / experts >= 16 || ff > DOWN_FF;
+    if (many) {
+        const int max_tiles = pairs / PLACES + std::min(pairs, experts);
+        const size_t g_up = blocks_of(ff) * max_tiles, g_down = (size_t)((width + 255) / 256) * max_tiles;
+        IFA_REQUIRE(g_up < (1u << 31) && g_down < (1u << 31), "ifa_moe_experts_fp8: too many rows");
+        int *counts = (int *)(base + W.counts);
+        hipLaunchKernelGGL(k_moe_fp8_count, dim3(W.blocks), dim3(1024), 0, st, idx_dev, pairs, experts, W.per, counts);
+        hipLaunchKernelGGL(k_moe_fp8_place, dim3(W.blocks), dim3(1024), 0, st, idx_dev, pairs, experts, top, PLACES, W.per, counts, place_row, pair_at, tiles, n_tiles);
+        const auto fn = wide ? k_moe_fp8_down_tile<true> : k_moe_fp8_down_tile<false>;
+        IFA_HIP_CHECK(hipFuncSetAttribute((const void *)k_moe_fp8_up_tile, hipFuncAttributeMaxDynamicSharedMemorySize, MoeTile::SMEM));
+        IFA_HIP_CHECK(hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, MoeTile::SMEM));
+        hipLaunchKernelGGL(k_moe_fp8_up_tile, dim3((unsigned)g_up), dim3(256), MoeTile::SMEM, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, (const uint8_t *)a_e4m3,
+                           lda, (const float *)a_scale_f32, lds, place_row, tiles, n_tiles, glu_kind, limit, q, s);
+        hipLaunchKernelGGL(fn, dim3((unsigned)g_down), dim3(256), MoeTile::SMEM, st, (const uint8_t *)down_e4m3, (const float *)down_scale_f32, width, ff, q, s, tiles, n_tiles, out);
+    } else {
+        hipLaunchKernelGGL(k_moe_fp8_up_list, dim3(ff / 16, experts), dim3(64 * LIST_WAVES), 0, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, pairs, top,
+                           (const uint8_t *)a_e4m3, lda, (const float *)a_scale_f32, lds, idx_dev, glu_kind, limit, act);
+        const auto fn = wide ? k_moe_fp8_down_list<true> : k_moe_fp8_down_list<false>;
+        const size_t list_lds = 16 * blocks_of(ff) * (BLOCK + 4);
+        IFA_HIP_CHECK(hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, 16 * DOWN_FF / BLOCK * (BLOCK + 4)));
+        hipLaunchKernelGGL(fn, dim3(ifa_cdiv(width, 16 * DOWN_WAVES), experts), dim3(64 * DOWN_WAVES), list_lds, st, (const uint8_t *)down_e4m3, (const float *)down_scale_f32, width, ff, pairs,
+                           idx_dev, act, out);
+        pair_at = nullptr;
+    }
     const size_t all = rows * (width / 4);
-#define IFA_JOIN(DT) hipLaunchKernelGGL((k_moe_fp8_join<DT>), dim3(ifa_cdiv(all, 256)), dim3(256), 0, st, out, pair_at, (const float *)wgt_f32, top, width, all, (Elem<DT>::type *)y, ldy, accumulate)
+#define IFA_JOIN(DT) hipLaunchKernelGGL((k_moe_fp8_join<DT>), dim3(ifa_cdiv(all, 256)), dim3(256), 0, st, out, pair_at, idx_dev, experts, (const float *)wgt_f32, top, width, all, (Elem<DT>::type *)y, ldy, \
+                                        accumulate)
     if (y_dtype == IFA_F32) IFA_JOIN(IFA_F32); else if (y_dtype == IFA_F16) IFA_JOIN(IFA_F16); else IFA_JOIN(IFA_BF16);
 #undef IFA_JOIN
     IFA_LAUNCH_CHECK();
