@@ -13,7 +13,7 @@ __device__ __forceinline__ void stream_blocks(const uint8_t *const (&w)[MATS], c
 {
     const int lane = threadIdx.x & 63, k_lane = 16 * (lane >> 4), whole = cols / BLOCK;
     struct Group { u32x4 w[DEPTH][MATS][2], a[DEPTH][TILES][2]; float sw[DEPTH][MATS], sa[DEPTH][TILES]; };
-    auto ask = [&](Group &G, int kb0) {          // (past the last whole block: the last one again, not used)
+    auto ask = [&](Group &G, int kb0) {          // (past the last whole block of a last group: that block again, not used)
 #pragma unroll
         for (int d = 0; d < DEPTH; d++) {
             const int kb = min(kb0 + d * step, whole - 1);
@@ -52,20 +52,25 @@ __device__ __forceinline__ void stream_blocks(const uint8_t *const (&w)[MATS], c
         }
     };
     if (first < whole) {
+        // a group asked for while the one before it is multiplied, none beyond the last (a request that may or may not have gone out would have the compiler wait for all: the ends stand apart)
         Group G[2];
-        ask(G[0], first);
-        int kb = first;
-        while (true) {
-            ask(G[1], kb + DEPTH * step);
+        const int groups = (whole - first + DEPTH * step - 1) / (DEPTH * step);
+        auto at = [&](int g) { return first + g * DEPTH * step; };
+        auto go = [&](const Group &X, int g) {
 #pragma unroll
-            for (int d = 0; d < DEPTH; d++) if (kb + d * step < whole) one(G[0].w[d], G[0].a[d], G[0].sw[d], G[0].sa[d]);
-            kb += DEPTH * step;
-            if (kb >= whole) break;
-            ask(G[0], kb + DEPTH * step);
-#pragma unroll
-            for (int d = 0; d < DEPTH; d++) if (kb + d * step < whole) one(G[1].w[d], G[1].a[d], G[1].sw[d], G[1].sa[d]);
-            kb += DEPTH * step;
-            if (kb >= whole) break;
+            for (int d = 0; d < DEPTH; d++) if (at(g) + d * step < whole) one(X.w[d], X.a[d], X.sw[d], X.sa[d]);
+        };
+        ask(G[0], at(0));
+        if (groups == 1) go(G[0], 0);
+        else {
+            ask(G[1], at(1));
+            int g = 0;
+            while (true) {
+                if (g + 2 >= groups) { go(G[0], g); go(G[1], g + 1); break; }
+                go(G[0], g); ask(G[0], at(g + 2)); g++;
+                if (g + 2 >= groups) { go(G[1], g); go(G[0], g + 1); break; }
+                go(G[1], g); ask(G[1], at(g + 2)); g++;
+            }
         }
     }
     if (whole * BLOCK < cols && whole % step == first) {          // the part of a block behind them

@@ -3,8 +3,10 @@
 //     c ^ ((r >> 1) & 7), so that sixteen lanes that read one piece of sixteen rows meet no bank twice (the permutation sits in the requests' source addresses);
 //   * a wave multiplies (BM / WM) x (BN / WN) values of a block as 16 x 16 products over all its 128 columns and adds each, times the two scales, to its 32-bit sums: four
 //     multiply-adds beside the 32 cycles of a product;
+//   * a buffer is asked for again in two parts, each as soon as everybody has read it: the activations, the scales and the matrix rows of a wave's first products in the middle of the block, the
+//     other matrix rows at its end.  So every request has one and a half blocks' products to arrive under (one block's: 2.1 us a block of a 256 x 256 tile, however few the tiles);
 //   * the requests are inline assembly without results (the compiler would wait for all of them in front of every read of LDS); the waits and barriers stand beside them.
-// Columns beyond the last block's end: the requests stay inside their row, and both operands' values there are taken as zero.  Rows beyond the last: repeated, not stored.
+// Columns beyond the last block's end: the requests stay inside their row, and zeros are written over what they brought.  Rows beyond the last: repeated, not stored.
 #pragma once
 #include "ifa_fp8.h"
 
@@ -12,120 +14,189 @@ namespace ifa8 {
 
 typedef __attribute__((address_space(3))) char lds_char;
 
-// 64 lanes' 16 bytes each to 1024 consecutive bytes of LDS from `to` (the same in all lanes); arrive behind arrive_all()
-__device__ __forceinline__ void request16(const void *from, uint32_t to)
+// 64 lanes' 16 bytes each to 1024 consecutive bytes of LDS from `to` (the same in all lanes), if `on` (the same in all lanes) is not 0 -- a branch inside, so that the compiler sees none and keeps
+// the products around it in their order; they have arrived behind arrive<n>() where n younger requests of the wave may be under way
+__device__ __forceinline__ void request16(const void *from, uint32_t to, int on)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "m0");
+    asm volatile("s_cmp_eq_u32 %2, 0\n\ts_cbranch_scc1 .Lrequest%=\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n.Lrequest%=:" ::"s"(to), "v"(from), "s"(__builtin_amdgcn_readfirstlane(on)) : "scc");
 }
-__device__ __forceinline__ void request16(const void *base, uint32_t offset, uint32_t to)      // (base: the same in all lanes)
+__device__ __forceinline__ void request16(const void *base, uint32_t offset, uint32_t to, int on)      // (base: the same in all lanes)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "m0");
+    asm volatile("s_cmp_eq_u32 %3, 0\n\ts_cbranch_scc1 .Lrequest%=\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n.Lrequest%=:" ::"s"(to), "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(on))
+                 : "scc");
 }
-__device__ __forceinline__ void arrive_all()      // this wave's requests are in LDS, then everybody's
+__device__ __forceinline__ void request4(const void *from, uint32_t to, int on)      // 64 lanes' 4 bytes each to 256 bytes
 {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_cmp_eq_u32 %2, 0\n\ts_cbranch_scc1 .Lrequest%=\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n.Lrequest%=:" ::"s"(to), "v"(from), "s"(__builtin_amdgcn_readfirstlane(on)) : "scc");
 }
+template <int N> __device__ __forceinline__ void arrive()      // this wave's requests but the last N, and everybody's; everybody's reads of LDS in front of it are done
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 __device__ __forceinline__ int slot_of(int row, int piece) { return piece ^ ((row >> 1) & 7); }
 
 template <int BM, int BN, int WM, int WN> struct Tile {
-    static constexpr int WAVES = WM * WN, TM = BM / (16 * WM), TN = BN / (16 * WN), WI = BM / (8 * WAVES), AI = BN / (8 * WAVES), BUF = (BM + BN) * BLOCK, SMEM = 2 * BUF;
+    static constexpr int WAVES = WM * WN, TM = BM / (16 * WM), TN = BN / (16 * WN), WI = BM / (8 * WAVES), AI = BN / (8 * WAVES), BUF = (BM + BN) * BLOCK, SCALES = 2 * 256 * WAVES;
+    static constexpr int SMEM = 2 * BUF + 2 * SCALES;          // two buffers; for each the waves' activation scales, then their matrix scales
     static_assert(WI * 8 * WAVES == BM && AI * 8 * WAVES == BN && TM * 16 * WM == BM && TN * 16 * WN == BN, "whole rows and products a wave");
+    static_assert(WI % 2 == 0 && TM % 2 == 0 && TM >= 4 && (BM / (16 * WM)) % 4 == 0 && TN <= 4 && BM == 128 * WM || BM == 64 * WM, "halves of a wave's matrix rows");
 };
 
-// One tile's sums.  The tile's matrix rows are wbase + woff(r), its activation rows asrc(r); wrow(m): the first of the 16 tile rows of product m of this wave; sw(m, b): the matrix scale of that
-// product's rows in block b (ONE_SCALE: the same for all m); sa: of activation row `lane` of this wave's (a lane below 16 TN).
-// The sums of a block are taken over one group of products behind it (p), so that no multiply-add waits for the product in front of it.
-template <bool WIDE, bool ONE_SCALE, class T, class WOff, class ASrc, class WRow, class SW>
-__device__ __forceinline__ void tile_sums(char *smem, int cols, const uint8_t *wbase, WOff woff, ASrc asrc, WRow wrow, SW sw, const float *sa, int arow0, f32x4 (&acc)[T::TM][T::TN])
+// One tile's sums.  The tile's matrix rows are wbase + woff(r), its activation rows asrc(r) (A32: abase + asrc(r), 32 bits).  Wave (wm, wn)'s products m = 0 .. TM - 1 have matrix rows
+// wm BM / WM + 16 m on; NSC 2: in two halves, m < TM / 2 from the tile's rows wm BM / (2 WM) on, the others BM / 2 further on, with matrix scales of their own.  sw(h): the row of block scales of half h;
+// sa: that of the lane's activation row (lane below 16 TN of this wave's).
+// A block's products (each over the wave's TN activation tiles) run without a break from block to block: a product's sums are taken in front of the one that takes its registers, TN products later.  The
+// barrier at a block's end stands in front of its last product, whose operands are read by then: under it the next block's first operands come from LDS.
+template <bool WIDE, int NSC, bool A32, class T, int WM, class WOff, class ASrc, class SW>
+__device__ __forceinline__ void tile_sums(char *smem, int cols, const uint8_t *wbase, WOff woff, const uint8_t *abase, ASrc asrc, SW sw, const float *sa, f32x4 (&acc)[T::TM][T::TN])
 {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int WROWS = T::WI * 8 * T::WAVES, AROWS = T::AI * 8 * T::WAVES, WH = T::WI / 2, FIRST = T::AI + WH + 2;          // requests of a block's first part; WH of the second
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % WM, wn = wave / WM;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char *)smem;
     const int nb = (cols + BLOCK - 1) / BLOCK, rest = cols - (nb - 1) * BLOCK;
-    uint32_t wo[T::WI];
-    const uint8_t *ap[T::AI];
-    constexpr int WROWS = T::WI * 8 * T::WAVES;
-    auto w_piece = [&](int j) { const int r = (wave * T::WI + j) * 8 + (lane >> 3); return 16 * slot_of(r, lane & 7); };
-    auto a_piece = [&](int j) { const int r = (wave * T::AI + j) * 8 + (lane >> 3); return 16 * slot_of(r, lane & 7); };
-#pragma unroll
-    for (int j = 0; j < T::WI; j++) wo[j] = woff((wave * T::WI + j) * 8 + (lane >> 3)) + w_piece(j);
-#pragma unroll
-    for (int j = 0; j < T::AI; j++) ap[j] = asrc((wave * T::AI + j) * 8 + (lane >> 3)) + a_piece(j);
-    auto request = [&](int b, uint32_t to) {
-        if (b + 1 < nb || rest == BLOCK) {
-#pragma unroll
-            for (int j = 0; j < T::WI; j++) request16(wbase + (size_t)b * BLOCK, wo[j], to + (wave * T::WI + j) * 1024);
-#pragma unroll
-            for (int j = 0; j < T::AI; j++) request16(ap[j] + (size_t)b * BLOCK, to + WROWS * BLOCK + (wave * T::AI + j) * 1024);
-        } else {
-#pragma unroll
-            for (int j = 0; j < T::WI; j++) request16(wbase + (size_t)b * BLOCK, wo[j] - max(0, w_piece(j) + 16 - rest), to + (wave * T::WI + j) * 1024);
-#pragma unroll
-            for (int j = 0; j < T::AI; j++) request16(ap[j] + (size_t)b * BLOCK - max(0, a_piece(j) + 16 - rest), to + WROWS * BLOCK + (wave * T::AI + j) * 1024);
-        }
+    // the rows of product m of wave row k: wrow(k, m) on.  Which rows a wave asks for: of its WI requests of 8 rows the first WH are of the first half of somebody's products
+    auto wrow = [&](int k, int m) { return NSC == 1 ? k * (WROWS / WM) + 16 * m : (m < T::TM / 2 ? 0 : WROWS / 2) + k * (WROWS / (2 * WM)) + 16 * (m % (T::TM / 2)); };
+    auto w_row8 = [&](int j) {          // the first of the 8 rows of request j
+        const int u = wave * WH + j % WH, k = u / T::TM, r = u % T::TM;          // (TM requests of 8 rows are half of a wave row's products)
+        return wrow(k, (j / WH) * (T::TM / 2) + r / 2) + 8 * (r & 1);
     };
-    const int i = lane & 15, g = lane >> 4;
-    auto read = [&](const char *image, int row, int k_end) {      // the lane's pieces g and g + 4 of a row
-        const char *at = image + row * BLOCK;
-        u32x4 lo = *reinterpret_cast<const u32x4 *>(at + 16 * slot_of(row, g)), hi = *reinterpret_cast<const u32x4 *>(at + 16 * slot_of(row, g + 4));
-        const u32x4 zero = {0u, 0u, 0u, 0u};
-        if (k_end < BLOCK) { if (16 * g >= k_end) lo = zero; if (16 * g + 64 >= k_end) hi = zero; }
+    uint32_t wo[T::WI], ao[A32 ? T::AI : 1];
+    const uint8_t *ap[A32 ? 1 : T::AI];
+    const int sub = lane >> 3;
+#pragma unroll
+    for (int j = 0; j < T::WI; j++) { const int r = w_row8(j) + sub; wo[j] = woff(r) + 16 * slot_of(r, lane & 7); }
+#pragma unroll
+    for (int j = 0; j < T::AI; j++) {
+        const int r = (wave * T::AI + j) * 8 + sub;
+        if constexpr (A32) ao[j] = asrc(r) + 16 * slot_of(r, lane & 7);
+        else ap[j] = asrc(r) + 16 * slot_of(r, lane & 7);
+    }
+    const float *const swl = sw(lane & (NSC - 1));
+    // in front of the last block's requests: pieces beyond the rows' end are their last one instead
+    auto draw_back = [&]() {
+        auto back = [&](int r) { return (uint32_t)max(0, 16 * slot_of(r, lane & 7) + 16 - rest); };
+#pragma unroll
+        for (int j = 0; j < T::WI; j++) wo[j] -= back(w_row8(j) + sub);
+#pragma unroll
+        for (int j = 0; j < T::AI; j++) { if constexpr (A32) ao[j] -= back((wave * T::AI + j) * 8 + sub); else ap[j] -= back((wave * T::AI + j) * 8 + sub); }
+    };
+    const uint32_t sc0 = lds0 + 2 * T::BUF + wave * 256;
+    auto ask_first = [&](int b, int k, int on) {          // request k of FIRST
+        if (k == 0) request4(sa + b, sc0 + (b & 1) * T::SCALES, on);
+        else if (k == 1) request4(swl + b, sc0 + (b & 1) * T::SCALES + T::SCALES / 2, on);
+        else if (k < 2 + T::AI) {
+            const int j = k - 2;
+            const uint32_t to = lds0 + (b & 1) * T::BUF + WROWS * BLOCK + (wave * T::AI + j) * 1024;
+            if constexpr (A32) request16(abase + (size_t)b * BLOCK, ao[j], to, on);
+            else request16(ap[j] + (size_t)b * BLOCK, to, on);
+        } else request16(wbase + (size_t)b * BLOCK, wo[k - 2 - T::AI], lds0 + (b & 1) * T::BUF + w_row8(k - 2 - T::AI) * BLOCK, on);
+    };
+    auto ask_second = [&](int b, int k, int on) { request16(wbase + (size_t)b * BLOCK, wo[WH + k], lds0 + (b & 1) * T::BUF + w_row8(WH + k) * BLOCK, on); };
+    auto ask = [&](int b) {
+        if (b + 1 == nb && rest < BLOCK) draw_back();
+#pragma unroll
+        for (int k = 0; k < FIRST; k++) ask_first(b, k, 1);
+#pragma unroll
+        for (int k = 0; k < WH; k++) ask_second(b, k, 1);
+    };
+    auto clear = [&](int b, bool second) {          // (the last block's columns that are none; everybody's requests of this part have arrived)
+        if (b + 1 < nb || rest == BLOCK) return;
+        char *const buf = smem + (b & 1) * T::BUF;
+        for (int k = threadIdx.x; k < (WROWS / 2 + (second ? 0 : AROWS)) * 8; k += 64 * T::WAVES) {
+            const int q = k >> 3, half = WROWS / 2, u = q / 8, r = q < half ? wrow(u / T::TM, (second ? T::TM / 2 : 0) + u % T::TM / 2) + 8 * (u & 1) + (q & 7) : WROWS + q - half;
+            if (16 * (k & 7) >= rest) *reinterpret_cast<u32x4 *>(buf + r * BLOCK + 16 * slot_of(r < WROWS ? r : r - WROWS, k & 7)) = u32x4{0u, 0u, 0u, 0u};
+        }
+        lds_barrier();
+    };
+    const int i = lane & 15, g = lane >> 4, piece = i * BLOCK + 16 * slot_of(i, g);          // (a product's rows start at multiples of 16: their slots are those of 0 .. 15)
+    auto read = [&](const char *rows16) {      // the lane's pieces g and g + 4 of its row
         Operand<WIDE> o;
-        o.set(lo, hi);
+        o.set(*reinterpret_cast<const u32x4 *>(rows16 + piece), *reinterpret_cast<const u32x4 *>(rows16 + (piece ^ 64)));
         return o;
     };
-    auto block = [&](const char *buf, int b, int k_end, float scale) {
-        Operand<WIDE> av[T::TN];
-        float s[T::TN];
+    Operand<WIDE> av[T::TN], wq[2];          // (a product's matrix rows are asked for two products ahead)
+    f32x4 p[T::TN];
+    float s[NSC][T::TN], last[T::TN];          // the scales of this block and, for its last product, of the one before
+    auto read_scales = [&](int b) {
+        const float *at = reinterpret_cast<const float *>(smem + 2 * T::BUF + (b & 1) * T::SCALES + wave * 256);
 #pragma unroll
-        for (int j = 0; j < T::TN; j++) {
-            av[j] = read(buf + WROWS * BLOCK, arow0 + 16 * j + i, k_end);
-            s[j] = __shfl(scale, 16 * j + i, 64);
-            if (ONE_SCALE) s[j] *= sw(0, b);
-        }
-        Operand<WIDE> wnext = read(buf, wrow(0) + i, k_end);
-        f32x4 p[2][T::TN];
-        auto add = [&](int m, int j) {
-            const float f = ONE_SCALE ? s[j] : s[j] * sw(m, b);
+        for (int h = 0; h < NSC; h++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) acc[m][j][r] = fmaf(p[m & 1][j][r], f, acc[m][j][r]);
-        };
+            for (int j = 0; j < T::TN; j++) s[h][j] = at[16 * j + i] * at[T::SCALES / 8 + h];
+    };
+    auto add = [&](int m, int j, float f) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) acc[m][j][r] = fmaf(p[j][r], f, acc[m][j][r]);
+        asm volatile("" : "+v"(acc[m][j]));          // (here: the compiler takes them behind the next branch otherwise, the products kept in registers until then)
+    };
+    const int arow = WROWS * BLOCK + wn * T::TN * 16 * BLOCK;
+    ask(0);
+    if (nb > 1) { ask(1); arrive<FIRST + WH>(); }
+    else arrive<0>();
+    clear(0, false);
+    clear(0, true);
+#pragma unroll
+    for (int j = 0; j < T::TN; j++) av[j] = read(smem + arow + 16 * j * BLOCK);
+    wq[0] = read(smem + wrow(wm, 0) * BLOCK);
+    wq[1] = read(smem + wrow(wm, 1) * BLOCK);
+    read_scales(0);
+#pragma unroll
+    for (int j = 0; j < T::TN; j++) { last[j] = 0.0f; p[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
+    // Product m reads the rows of product m + 2 behind itself; the middle of a block is MID, where the first half's rows are read and the second's are about to be, its end END, the same the other way
+    // round (their barriers stand inside the products, so that the reads before have time to arrive).  Between MID and END the requests of a block's first part go out, one beside a product, behind
+    // END those of the second.
+    constexpr int MID = T::TM / 2 - 2, END = T::TM - 2, SLOTS = (END - MID - 1) * T::TN, EACH = (FIRST + SLOTS - 1) / SLOTS, EACH2 = (WH + T::TN - 1) / T::TN;
+    for (int b = 0; b < nb; b++) {
+        const char *const cur = smem + (b & 1) * T::BUF, *const nxt = smem + (~b & 1) * T::BUF;
+        const int more = b + 2 < nb;
 #pragma unroll
         for (int m = 0; m < T::TM; m++) {
-            const Operand<WIDE> wv = wnext;
-            if (m + 1 < T::TM) wnext = read(buf, wrow(m + 1) + i, k_end);
+            const Operand<WIDE> wv = wq[m & 1];
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int j = 0; j < T::TN; j++) {
-                p[m & 1][j] = mfma128(wv, av[j]);
-                if (m > 0) add(m - 1, j);
+                if (m == MID && j == T::TN / 2) {          // the block's second part is there; its first one is read, scales and activations too
+                    if (b + 1 < nb) arrive<FIRST + WH>(); else arrive<0>();
+                    if (b > 0) clear(b, true);
+                    if (b + 3 == nb && rest < BLOCK) draw_back();
+                }
+                if (m == END && j == T::TN / 2) {          // the next block's first part is there; this one's second is read
+                    if (b + 2 < nb) arrive<FIRST + WH>();
+                    else if (b + 1 < nb) { arrive<WH>(); clear(b + 1, false); }
+                }
+                if (m > 0) add(m - 1, j, s[m - 1 < T::TM / 2 ? 0 : NSC - 1][j]);
+                else add(T::TM - 1, j, last[j]);
+                p[j] = mfma128(wv, av[j]);
+                if (m + 1 == T::TM) av[j] = read(nxt + arow + 16 * j * BLOCK);          // (behind the last block: what is there, not used)
+                if (j == T::TN - 1) wq[m & 1] = m + 2 < T::TM ? read(cur + wrow(wm, m + 2) * BLOCK) : read(nxt + wrow(wm, m + 2 - T::TM) * BLOCK);
+                if (m > MID && m < END) {
+#pragma unroll
+                    for (int k = ((m - MID - 1) * T::TN + j) * EACH; k < ((m - MID - 1) * T::TN + j + 1) * EACH; k++) if (k < FIRST) ask_first(b + 2, k, more);
+                } else if (m > END) {
+#pragma unroll
+                    for (int k = ((m - END - 1) * T::TN + j) * EACH2; k < ((m - END - 1) * T::TN + j + 1) * EACH2; k++) if (k < WH) ask_second(b + 2, k, more);
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
 #pragma unroll
-        for (int j = 0; j < T::TN; j++) add(T::TM - 1, j);
-    };
-    float scale = sa[0];
-    request(0, lds0);
-    arrive_all();
-    for (int b = 0; b + 1 < nb; b++) {
-        const float next = sa[b + 1];
-        request(b + 1, lds0 + ((b + 1) & 1) * T::BUF);
-        block(smem + (b & 1) * T::BUF, b, BLOCK, scale);
-        scale = next;
-        arrive_all();
+        for (int j = 0; j < T::TN; j++) last[j] = s[NSC - 1][j];
+        read_scales(b + 1);
     }
-    block(smem + ((nb - 1) & 1) * T::BUF, nb - 1, rest, scale);
+#pragma unroll
+    for (int j = 0; j < T::TN; j++) add(T::TM - 1, j, last[j]);
 }
 
 // A wave's sums by way of LDS, so that they leave in whole lines: f(t, n, v) with N consecutive values of activation row t from matrix row n on (both counted from the wave's first).  Every wave
 // has its part of the buffers; all of them are through with the last block.
 template <class T, int N, class F> __device__ __forceinline__ void tile_out(char *smem, const f32x4 (&acc)[T::TM][T::TN], F f)
 {
-    constexpr int PART = T::SMEM / T::WAVES, ROW = T::TM * 64, ROWS = PART / ROW / 16 * 16 < T::TN * 16 ? PART / ROW / 16 * 16 : T::TN * 16, PIECES = T::TM * 4;      // 16-byte pieces a row
+    constexpr int PART = 2 * T::BUF / T::WAVES, ROW = T::TM * 64, ROWS = PART / ROW / 16 * 16 < T::TN * 16 ? PART / ROW / 16 * 16 : T::TN * 16, PIECES = T::TM * 4;      // 16-byte pieces a row
     static_assert(ROWS >= 16 && (PIECES & (PIECES - 1)) == 0 && PIECES >= 16, "a part of 16 rows at least");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     char *const part = smem + wave * PART;
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    lds_barrier();
 #pragma unroll
     for (int t0 = 0; t0 < T::TN * 16; t0 += ROWS) {
 #pragma unroll
@@ -140,6 +211,7 @@ template <class T, int N, class F> __device__ __forceinline__ void tile_out(char
             const int t = k / LANES, c = k % LANES;
             if (t0 + t >= T::TN * 16) break;
             float v[N];
+            if constexpr (N == 1) v[0] = *reinterpret_cast<const float *>(part + t * ROW + 16 * ((c >> 2) ^ (t & 15)) + 4 * (c & 3));
 #pragma unroll
             for (int q = 0; q < N / 4; q++) {
                 const f32x4 x = *reinterpret_cast<const f32x4 *>(part + t * ROW + 16 * ((c * (N / 4) + q) ^ (t & 15)));

@@ -449,8 +449,8 @@ __global__ void __launch_bounds__(1024) k_moe_fp8_place(const int *__restrict__ 
 }
 
 // Tiles of 64 places of one expert.  A workgroup of four waves, two a compute unit.
-constexpr int PLACES = 64;
-typedef Tile<256, PLACES, 2, 2> MoeTile;
+constexpr int PLACES = 128;
+typedef Tile<256, PLACES, 2, PLACES / 32> MoeTile;
 
 // the tile's place among those that there are (the empty ones behind them are dealt to nobody); tiles of one expert side by side
 __device__ __forceinline__ bool moe_tile(const int *n_tiles, int blocks, int &tile, int &block)
@@ -465,7 +465,7 @@ __device__ __forceinline__ bool moe_tile(const int *n_tiles, int blocks, int &ti
 }
 
 // a tile of 128 gate rows and the 128 up rows of the same columns: one block of the activations, which leave it quantised
-__global__ void __launch_bounds__(256, 2) k_moe_fp8_up_tile(const uint8_t *__restrict__ gu, const float *__restrict__ sgu, int width, int ff, const uint8_t *__restrict__ a, size_t lda,
+__global__ void __launch_bounds__(64 * MoeTile::WAVES, 2) k_moe_fp8_up_tile(const uint8_t *__restrict__ gu, const float *__restrict__ sgu, int width, int ff, const uint8_t *__restrict__ a, size_t lda,
                                                             const float *__restrict__ sa, size_t lds, const int *__restrict__ place_row, const int *__restrict__ tiles,
                                                             const int *__restrict__ n_tiles, int kind, float limit, uint8_t *__restrict__ q, float *__restrict__ s)
 {
@@ -483,11 +483,10 @@ __global__ void __launch_bounds__(256, 2) k_moe_fp8_up_tile(const uint8_t *__res
     const size_t wb = blocks_of(width);
     const float *sg = sgu + ((size_t)e * 2 * fb + block) * wb, *su = sg + fb * wb;
     auto row_of = [&](int r) { return (size_t)place_row[at0 + min(r, n_at - 1)]; };
-    tile_sums<false, false, T>(
-        smem, width, gu + (size_t)e * 2 * ff * width, [&](int r) { return (uint32_t)((r < BLOCK ? 0 : ff) + min(n0 + (r & (BLOCK - 1)), ff - 1)) * (uint32_t)width; },
-        [&](int r) { return a + row_of(r) * lda; }, [&](int m) { return (m < 4 ? 0 : BLOCK) + 64 * wm + 16 * (m & 3); }, [&](int m, int b) { return m < 4 ? sg[b] : su[b]; },
-        sa + row_of(32 * wn + (lane & 31)) * lds, 32 * wn, acc);
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");          // (the buffers' last block is read)
+    tile_sums<false, 2, false, T, 2>(
+        smem, width, gu + (size_t)e * 2 * ff * width, [&](int r) { return (uint32_t)((r < BLOCK ? 0 : ff) + min(n0 + (r & (BLOCK - 1)), ff - 1)) * (uint32_t)width; }, nullptr,
+        [&](int r) { return a + row_of(r) * lda; }, [&](int h) { return h ? su : sg; }, sa + row_of(32 * wn + (lane & 31)) * lds, acc);
+    lds_barrier();          // (the buffers' last block is read)
     uint32_t *const most = reinterpret_cast<uint32_t *>(smem + PLACES * BLOCK);          // [2 waves][64 places], behind the tile's quantised rows
     const bool whole = n0 + BLOCK <= ff;
     uint32_t mine[T::TN];
@@ -521,14 +520,14 @@ __global__ void __launch_bounds__(256, 2) k_moe_fp8_up_tile(const uint8_t *__res
     }
     __syncthreads();
 #pragma unroll
-    for (int k = threadIdx.x; k < PLACES * 8; k += 256) {
+    for (int k = threadIdx.x; k < PLACES * 8; k += 64 * T::WAVES) {
         const int at = k >> 3, piece = k & 7;
         if (at < n_at && n0 + 16 * piece < ff) *reinterpret_cast<u32x4 *>(q + (size_t)(at0 + at) * ff + n0 + 16 * piece) = *reinterpret_cast<const u32x4 *>(smem + at * BLOCK + 16 * (piece ^ (at & 7)));
     }
 }
 
 template <bool WIDE>
-__global__ void __launch_bounds__(256, 2) k_moe_fp8_down_tile(const uint8_t *__restrict__ down, const float *__restrict__ sdown, int width, int ff, const uint8_t *__restrict__ q,
+__global__ void __launch_bounds__(64 * MoeTile::WAVES, 2) k_moe_fp8_down_tile(const uint8_t *__restrict__ down, const float *__restrict__ sdown, int width, int ff, const uint8_t *__restrict__ q,
                                                               const float *__restrict__ s, const int *__restrict__ tiles, const int *__restrict__ n_tiles, float *__restrict__ out)
 {
     typedef MoeTile T;
@@ -545,10 +544,9 @@ __global__ void __launch_bounds__(256, 2) k_moe_fp8_down_tile(const uint8_t *__r
     const size_t wb = blocks_of(width), fb = blocks_of(ff);
     const int nw = n0 + 128 * wm;
     const float *sd = sdown + ((size_t)e * wb + min(nw, width - 1) / BLOCK) * fb;
-    tile_sums<WIDE, true, T>(
-        smem, ff, down + ((size_t)e * width + n0) * ff, [&](int r) { return (uint32_t)min(r, width - 1 - n0) * (uint32_t)ff; },
-        [&](int r) { return q + (size_t)(at0 + min(r, n_at - 1)) * ff; }, [&](int m) { return 128 * wm + 16 * m; }, [&](int, int b) { return sd[b]; },
-        s + (size_t)(at0 + min(32 * wn + (lane & 31), n_at - 1)) * fb, 32 * wn, acc);
+    tile_sums<WIDE, 1, true, T, 2>(
+        smem, ff, down + ((size_t)e * width + n0) * ff, [&](int r) { return (uint32_t)min(r, width - 1 - n0) * (uint32_t)ff; }, q + (size_t)at0 * ff,
+        [&](int r) { return (uint32_t)min(r, n_at - 1) * (uint32_t)ff; }, [&](int) { return sd; }, s + (size_t)(at0 + min(32 * wn + (lane & 31), n_at - 1)) * fb, acc);
     tile_out<T, 4>(smem, acc, [&](int t, int n, float *v) {
         if (32 * wn + t < n_at && nw + n < width) *reinterpret_cast<u32x4 *>(out + (size_t)(at0 + 32 * wn + t) * width + nw + n) = pack<IFA_F32>(v);          // (width in whole 16s)
     });
@@ -672,9 +670,9 @@ int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t ld
         const auto fn = wide ? k_moe_fp8_down_tile<true> : k_moe_fp8_down_tile<false>;
         IFA_HIP_CHECK(hipFuncSetAttribute((const void *)k_moe_fp8_up_tile, hipFuncAttributeMaxDynamicSharedMemorySize, MoeTile::SMEM));
         IFA_HIP_CHECK(hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, MoeTile::SMEM));
-        hipLaunchKernelGGL(k_moe_fp8_up_tile, dim3((unsigned)g_up), dim3(256), MoeTile::SMEM, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, (const uint8_t *)a_e4m3,
+        hipLaunchKernelGGL(k_moe_fp8_up_tile, dim3((unsigned)g_up), dim3(64 * MoeTile::WAVES), MoeTile::SMEM, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, (const uint8_t *)a_e4m3,
                            lda, (const float *)a_scale_f32, lds, place_row, tiles, n_tiles, glu_kind, limit, q, s);
-        hipLaunchKernelGGL(fn, dim3((unsigned)g_down), dim3(256), MoeTile::SMEM, st, (const uint8_t *)down_e4m3, (const float *)down_scale_f32, width, ff, q, s, tiles, n_tiles, out);
+        hipLaunchKernelGGL(fn, dim3((unsigned)g_down), dim3(64 * MoeTile::WAVES), MoeTile::SMEM, st, (const uint8_t *)down_e4m3, (const float *)down_scale_f32, width, ff, q, s, tiles, n_tiles, out);
     } else {
         hipLaunchKernelGGL(k_moe_fp8_up_list, dim3(ff / 16, experts), dim3(64 * LIST_WAVES), 0, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, pairs, top,
                            (const uint8_t *)a_e4m3, lda, (const float *)a_scale_f32, lds, idx_dev, glu_kind, limit, act);
