@@ -221,8 +221,7 @@ int linear(const Product &P, hipStream_t s)
     }
     // sixteen waves where there is a workgroup for each compute unit at most: one row, 4096 x 4096 6.4 -> 5.5 us, 4096 x 11008 13.1 -> 12.7; 11008 x 4096 12.2 -> 13.2
     if (P.tokens <= 16) return P.rows <= 4096 && P.cols >= 16 * BLOCK ? launch_stream<DT, 1, 1, 16, 1>(P, s) : launch_stream<DT, 1, 1, 8, 1>(P, s);
-    // 32 matrix rows a workgroup where that leaves enough of them: the activations' way from the caches is as long as the matrix's from memory.  24 rows, 5632 x 2064 7.9 -> 7.2; 2048 x 2048 5.7 -> 7.2; 19 rows, 8275 x 928 6.1 -> 8.0
-    return P.rows >= 4096 && P.cols >= 16 * BLOCK ? launch_stream<DT, 2, 2, 8, 1>(P, s) : launch_stream<DT, 1, 2, 8, 1>(P, s);
+    return launch_stream<DT, 1, 2, 8, 1>(P, s);
 }
 
 } // namespace

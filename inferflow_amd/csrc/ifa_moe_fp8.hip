@@ -303,7 +303,7 @@ __device__ __forceinline__ void up_list(const uint16_t *list, int n, const uint8
         ar[j] = a + t * lda; sar[j] = sa + t * lds;
         acc[0][j] = acc[1][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    stream_blocks<false, 1, 2, TILES>(wr, swr, ar, sar, width, wave, LIST_WAVES, acc);
+    stream_blocks<false, 1, 2, TILES, false>(wr, swr, ar, sar, width, wave, LIST_WAVES, acc);
     join_waves<LIST_WAVES, 2, TILES>(acc, red);
     if (wave == 0) {
 #pragma unroll
