@@ -4,7 +4,8 @@
 //   * a wave multiplies (BM / WM) x (BN / WN) values of a block as 16 x 16 products over all its 128 columns and adds each, times the two scales, to its 32-bit sums: four
 //     multiply-adds beside the 32 cycles of a product;
 //   * a buffer is asked for again in two parts, each as soon as everybody has read it: the activations, the scales and the matrix rows of a wave's first products in the middle of the block, the
-//     other matrix rows at its end.  So every request has one and a half blocks' products to arrive under (one block's: 2.1 us a block of a 256 x 256 tile, however few the tiles);
+//     other matrix rows at its end.  So every request has one and a half blocks' products to arrive under (one block's: 2.1 us a block of a 256 x 256 tile instead of 1.8; two and a half, a third buffer
+//     of 256 x 128 tiles: 1.13 instead of 1.11);
 //   * the requests are inline assembly without results (the compiler would wait for all of them in front of every read of LDS); the waits and barriers stand beside them.
 // Columns beyond the last block's end: the requests stay inside their row, and zeros are written over what they brought.  Rows beyond the last: repeated, not stored.
 #pragma once
@@ -36,20 +37,21 @@ template <int N> __device__ __forceinline__ void arrive()      // this wave's re
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 __device__ __forceinline__ int slot_of(int row, int piece) { return piece ^ ((row >> 1) & 7); }
 
-template <int BM, int BN, int WM, int WN> struct Tile {
-    static constexpr int WAVES = WM * WN, TM = BM / (16 * WM), TN = BN / (16 * WN), WI = BM / (8 * WAVES), AI = BN / (8 * WAVES), BUF = (BM + BN) * BLOCK, SCALES = 2 * 256 * WAVES;
-    static constexpr int SMEM = 2 * BUF + 2 * SCALES;          // two buffers; for each the waves' activation scales, then their matrix scales
+template <int BM, int BN, int WM, int WN, int NST = 2> struct Tile {
+    static constexpr int STAGES = NST, WAVES = WM * WN, TM = BM / (16 * WM), TN = BN / (16 * WN), WI = BM / (8 * WAVES), AI = BN / (8 * WAVES), BUF = (BM + BN) * BLOCK, SCALES = 2 * 256 * WAVES;
+    static constexpr int SMEM = NST * (BUF + SCALES);          // the buffers; for each the waves' activation scales, then their matrix scales
     static_assert(WI * 8 * WAVES == BM && AI * 8 * WAVES == BN && TM * 16 * WM == BM && TN * 16 * WN == BN, "whole rows and products a wave");
     static_assert(WI % 2 == 0 && TM % 2 == 0 && TM >= 4 && (BM / (16 * WM)) % 4 == 0 && TN <= 4 && BM == 128 * WM || BM == 64 * WM, "halves of a wave's matrix rows");
 };
 
 // One tile's sums.  The tile's matrix rows are wbase + woff(r), its activation rows asrc(r) (A32: abase + asrc(r), 32 bits).  Wave (wm, wn)'s products m = 0 .. TM - 1 have matrix rows
 // wm BM / WM + 16 m on; NSC 2: in two halves, m < TM / 2 from the tile's rows wm BM / (2 WM) on, the others BM / 2 further on, with matrix scales of their own.  sw(h): the row of block scales of half h;
-// sa: that of the lane's activation row (lane below 16 TN of this wave's).
+// sa: that of the lane's activation row (lane below 16 TN of this wave's).  idle: none of the wave's activation rows is one: it asks for its part and waits with the others, no more (the chip is at its
+// power limit in the products).
 // A block's products (each over the wave's TN activation tiles) run without a break from block to block: a product's sums are taken in front of the one that takes its registers, TN products later.  The
 // barrier at a block's end stands in front of its last product, whose operands are read by then: under it the next block's first operands come from LDS.
 template <bool WIDE, int NSC, bool A32, class T, int WM, class WOff, class ASrc, class SW>
-__device__ __forceinline__ void tile_sums(char *smem, int cols, const uint8_t *wbase, WOff woff, const uint8_t *abase, ASrc asrc, SW sw, const float *sa, f32x4 (&acc)[T::TM][T::TN])
+__device__ __forceinline__ void tile_sums(char *smem, int cols, const uint8_t *wbase, WOff woff, const uint8_t *abase, ASrc asrc, SW sw, const float *sa, bool idle, f32x4 (&acc)[T::TM][T::TN])
 {
     constexpr int WROWS = T::WI * 8 * T::WAVES, AROWS = T::AI * 8 * T::WAVES, WH = T::WI / 2, FIRST = T::AI + WH + 2;          // requests of a block's first part; WH of the second
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % WM, wn = wave / WM;
@@ -81,28 +83,28 @@ __device__ __forceinline__ void tile_sums(char *smem, int cols, const uint8_t *w
 #pragma unroll
         for (int j = 0; j < T::AI; j++) { if constexpr (A32) ao[j] -= back((wave * T::AI + j) * 8 + sub); else ap[j] -= back((wave * T::AI + j) * 8 + sub); }
     };
-    const uint32_t sc0 = lds0 + 2 * T::BUF + wave * 256;
-    auto ask_first = [&](int b, int k, int on) {          // request k of FIRST
-        if (k == 0) request4(sa + b, sc0 + (b & 1) * T::SCALES, on);
-        else if (k == 1) request4(swl + b, sc0 + (b & 1) * T::SCALES + T::SCALES / 2, on);
+    const uint32_t sc0 = lds0 + T::STAGES * T::BUF + wave * 256;
+    auto ask_first = [&](int b, int slot, int k, int on) {          // request k of FIRST of block b into buffer `slot`
+        if (k == 0) request4(sa + b, sc0 + slot * T::SCALES, on);
+        else if (k == 1) request4(swl + b, sc0 + slot * T::SCALES + T::SCALES / 2, on);
         else if (k < 2 + T::AI) {
             const int j = k - 2;
-            const uint32_t to = lds0 + (b & 1) * T::BUF + WROWS * BLOCK + (wave * T::AI + j) * 1024;
+            const uint32_t to = lds0 + slot * T::BUF + WROWS * BLOCK + (wave * T::AI + j) * 1024;
             if constexpr (A32) request16(abase + (size_t)b * BLOCK, ao[j], to, on);
             else request16(ap[j] + (size_t)b * BLOCK, to, on);
-        } else request16(wbase + (size_t)b * BLOCK, wo[k - 2 - T::AI], lds0 + (b & 1) * T::BUF + w_row8(k - 2 - T::AI) * BLOCK, on);
+        } else request16(wbase + (size_t)b * BLOCK, wo[k - 2 - T::AI], lds0 + slot * T::BUF + w_row8(k - 2 - T::AI) * BLOCK, on);
     };
-    auto ask_second = [&](int b, int k, int on) { request16(wbase + (size_t)b * BLOCK, wo[WH + k], lds0 + (b & 1) * T::BUF + w_row8(WH + k) * BLOCK, on); };
-    auto ask = [&](int b) {
+    auto ask_second = [&](int b, int slot, int k, int on) { request16(wbase + (size_t)b * BLOCK, wo[WH + k], lds0 + slot * T::BUF + w_row8(WH + k) * BLOCK, on); };
+    auto ask = [&](int b) {          // (in front of the loop: b < STAGES)
         if (b + 1 == nb && rest < BLOCK) draw_back();
 #pragma unroll
-        for (int k = 0; k < FIRST; k++) ask_first(b, k, 1);
+        for (int k = 0; k < FIRST; k++) ask_first(b, b, k, 1);
 #pragma unroll
-        for (int k = 0; k < WH; k++) ask_second(b, k, 1);
+        for (int k = 0; k < WH; k++) ask_second(b, b, k, 1);
     };
-    auto clear = [&](int b, bool second) {          // (the last block's columns that are none; everybody's requests of this part have arrived)
+    auto clear = [&](int b, int slot, bool second) {          // (the last block's columns that are none; everybody's requests of this part have arrived)
         if (b + 1 < nb || rest == BLOCK) return;
-        char *const buf = smem + (b & 1) * T::BUF;
+        char *const buf = smem + slot * T::BUF;
         for (int k = threadIdx.x; k < (WROWS / 2 + (second ? 0 : AROWS)) * 8; k += 64 * T::WAVES) {
             const int q = k >> 3, half = WROWS / 2, u = q / 8, r = q < half ? wrow(u / T::TM, (second ? T::TM / 2 : 0) + u % T::TM / 2) + 8 * (u & 1) + (q & 7) : WROWS + q - half;
             if (16 * (k & 7) >= rest) *reinterpret_cast<u32x4 *>(buf + r * BLOCK + 16 * slot_of(r < WROWS ? r : r - WROWS, k & 7)) = u32x4{0u, 0u, 0u, 0u};
@@ -118,8 +120,8 @@ __device__ __forceinline__ void tile_sums(char *smem, int cols, const uint8_t *w
     Operand<WIDE> av[T::TN], wq[2];          // (a product's matrix rows are asked for two products ahead)
     f32x4 p[T::TN];
     float s[NSC][T::TN], last[T::TN];          // the scales of this block and, for its last product, of the one before
-    auto read_scales = [&](int b) {
-        const float *at = reinterpret_cast<const float *>(smem + 2 * T::BUF + (b & 1) * T::SCALES + wave * 256);
+    auto read_scales = [&](int slot) {
+        const float *at = reinterpret_cast<const float *>(smem + T::STAGES * T::BUF + slot * T::SCALES + wave * 256);
 #pragma unroll
         for (int h = 0; h < NSC; h++)
 #pragma unroll
@@ -131,11 +133,30 @@ __device__ __forceinline__ void tile_sums(char *smem, int cols, const uint8_t *w
         asm volatile("" : "+v"(acc[m][j]));          // (here: the compiler takes them behind the next branch otherwise, the products kept in registers until then)
     };
     const int arow = WROWS * BLOCK + wn * T::TN * 16 * BLOCK;
+    constexpr int YOUNGER = (T::STAGES - 1) * (FIRST + WH);          // requests behind those that a barrier waits for, as long as there are blocks to ask for
     ask(0);
-    if (nb > 1) { ask(1); arrive<FIRST + WH>(); }
-    else arrive<0>();
-    clear(0, false);
-    clear(0, true);
+#pragma unroll
+    for (int b = 1; b < T::STAGES; b++) if (b < nb) ask(b);
+    if (nb >= T::STAGES) arrive<YOUNGER>(); else arrive<0>();
+    clear(0, 0, false);
+    clear(0, 0, true);
+    int slot = 0;
+    if (idle) {
+        for (int b = 0; b < nb; b++) {
+            const int next = slot + 1 == T::STAGES ? 0 : slot + 1, more = b + T::STAGES < nb;
+            if (b + T::STAGES - 1 < nb) arrive<YOUNGER>(); else arrive<0>();
+            if (b > 0) clear(b, slot, true);
+            if (b + T::STAGES + 1 == nb && rest < BLOCK) draw_back();
+#pragma unroll
+            for (int k = 0; k < FIRST; k++) ask_first(b + T::STAGES, slot, k, more);
+            if (more) arrive<YOUNGER>();
+            else if (b + 1 < nb) { arrive<WH>(); clear(b + 1, next, false); }
+#pragma unroll
+            for (int k = 0; k < WH; k++) ask_second(b + T::STAGES, slot, k, more);
+            slot = next;
+        }
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < T::TN; j++) av[j] = read(smem + arow + 16 * j * BLOCK);
     wq[0] = read(smem + wrow(wm, 0) * BLOCK);
@@ -148,8 +169,9 @@ __device__ __forceinline__ void tile_sums(char *smem, int cols, const uint8_t *w
     // END those of the second.
     constexpr int MID = T::TM / 2 - 2, END = T::TM - 2, SLOTS = (END - MID - 1) * T::TN, EACH = (FIRST + SLOTS - 1) / SLOTS, EACH2 = (WH + T::TN - 1) / T::TN;
     for (int b = 0; b < nb; b++) {
-        const char *const cur = smem + (b & 1) * T::BUF, *const nxt = smem + (~b & 1) * T::BUF;
-        const int more = b + 2 < nb;
+        const int next = slot + 1 == T::STAGES ? 0 : slot + 1;
+        const char *const cur = smem + slot * T::BUF, *const nxt = smem + next * T::BUF;
+        const int more = b + T::STAGES < nb;
 #pragma unroll
         for (int m = 0; m < T::TM; m++) {
             const Operand<WIDE> wv = wq[m & 1];
@@ -157,13 +179,13 @@ __device__ __forceinline__ void tile_sums(char *smem, int cols, const uint8_t *w
 #pragma unroll
             for (int j = 0; j < T::TN; j++) {
                 if (m == MID && j == T::TN / 2) {          // the block's second part is there; its first one is read, scales and activations too
-                    if (b + 1 < nb) arrive<FIRST + WH>(); else arrive<0>();
-                    if (b > 0) clear(b, true);
-                    if (b + 3 == nb && rest < BLOCK) draw_back();
+                    if (b + T::STAGES - 1 < nb) arrive<YOUNGER>(); else arrive<0>();
+                    if (b > 0) clear(b, slot, true);
+                    if (b + T::STAGES + 1 == nb && rest < BLOCK) draw_back();
                 }
                 if (m == END && j == T::TN / 2) {          // the next block's first part is there; this one's second is read
-                    if (b + 2 < nb) arrive<FIRST + WH>();
-                    else if (b + 1 < nb) { arrive<WH>(); clear(b + 1, false); }
+                    if (b + T::STAGES < nb) arrive<YOUNGER>();
+                    else if (b + 1 < nb) { arrive<WH>(); clear(b + 1, next, false); }
                 }
                 if (m > 0) add(m - 1, j, s[m - 1 < T::TM / 2 ? 0 : NSC - 1][j]);
                 else add(T::TM - 1, j, last[j]);
@@ -172,17 +194,18 @@ __device__ __forceinline__ void tile_sums(char *smem, int cols, const uint8_t *w
                 if (j == T::TN - 1) wq[m & 1] = m + 2 < T::TM ? read(cur + wrow(wm, m + 2) * BLOCK) : read(nxt + wrow(wm, m + 2 - T::TM) * BLOCK);
                 if (m > MID && m < END) {
 #pragma unroll
-                    for (int k = ((m - MID - 1) * T::TN + j) * EACH; k < ((m - MID - 1) * T::TN + j + 1) * EACH; k++) if (k < FIRST) ask_first(b + 2, k, more);
+                    for (int k = ((m - MID - 1) * T::TN + j) * EACH; k < ((m - MID - 1) * T::TN + j + 1) * EACH; k++) if (k < FIRST) ask_first(b + T::STAGES, slot, k, more);
                 } else if (m > END) {
 #pragma unroll
-                    for (int k = ((m - END - 1) * T::TN + j) * EACH2; k < ((m - END - 1) * T::TN + j + 1) * EACH2; k++) if (k < WH) ask_second(b + 2, k, more);
+                    for (int k = ((m - END - 1) * T::TN + j) * EACH2; k < ((m - END - 1) * T::TN + j + 1) * EACH2; k++) if (k < WH) ask_second(b + T::STAGES, slot, k, more);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
 #pragma unroll
         for (int j = 0; j < T::TN; j++) last[j] = s[NSC - 1][j];
-        read_scales(b + 1);
+        read_scales(next);
+        slot = next;
     }
 #pragma unroll
     for (int j = 0; j < T::TN; j++) add(T::TM - 1, j, last[j]);
@@ -192,7 +215,7 @@ __device__ __forceinline__ void tile_sums(char *smem, int cols, const uint8_t *w
 // has its part of the buffers; all of them are through with the last block.
 template <class T, int N, class F> __device__ __forceinline__ void tile_out(char *smem, const f32x4 (&acc)[T::TM][T::TN], F f)
 {
-    constexpr int PART = 2 * T::BUF / T::WAVES, ROW = T::TM * 64, ROWS = PART / ROW / 16 * 16 < T::TN * 16 ? PART / ROW / 16 * 16 : T::TN * 16, PIECES = T::TM * 4;      // 16-byte pieces a row
+    constexpr int PART = T::STAGES * T::BUF / T::WAVES / 1024 * 1024, ROW = T::TM * 64, ROWS = PART / ROW / 16 * 16 < T::TN * 16 ? PART / ROW / 16 * 16 : T::TN * 16, PIECES = T::TM * 4;      // 16-byte pieces a row
     static_assert(ROWS >= 16 && (PIECES & (PIECES - 1)) == 0 && PIECES >= 16, "a part of 16 rows at least");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     char *const part = smem + wave * PART;

@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_linear_fp8_tile(const uint8
     tile_sums<DT == IFA_F32, 1, true, T, WM>(
         smem, min(cols, b1 * BLOCK) - b0 * BLOCK, w + (size_t)n0 * cols + (size_t)b0 * BLOCK, [&](int r) { return (uint32_t)min(r, rows - 1 - n0) * (uint32_t)cols; },
         a + (size_t)t0 * lda + (size_t)b0 * BLOCK, [&](int r) { return (uint32_t)min(r, tokens - 1 - t0) * (uint32_t)lda; }, [&](int) { return swr + b0; },
-        sa + (size_t)min(tw + lane % (16 * T::TN), tokens - 1) * lds + b0, acc);
+        sa + (size_t)min(tw + lane % (16 * T::TN), tokens - 1) * lds + b0, tw >= tokens || nw >= rows, acc);
     if (parts > 1) {
         float *const plane = planes + (size_t)part * tokens * rows;
         tile_out<T, 4>(smem, acc, [&](int t, int n, float *v) {

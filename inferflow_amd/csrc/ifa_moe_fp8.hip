@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(64 * MoeTile::WAVES, 2) k_moe_fp8_up_tile(cons
     auto row_of = [&](int r) { return (size_t)place_row[at0 + min(r, n_at - 1)]; };
     tile_sums<false, 2, false, T, 2>(
         smem, width, gu + (size_t)e * 2 * ff * width, [&](int r) { return (uint32_t)((r < BLOCK ? 0 : ff) + min(n0 + (r & (BLOCK - 1)), ff - 1)) * (uint32_t)width; }, nullptr,
-        [&](int r) { return a + row_of(r) * lda; }, [&](int h) { return h ? su : sg; }, sa + row_of(32 * wn + (lane & 31)) * lds, acc);
+        [&](int r) { return a + row_of(r) * lda; }, [&](int h) { return h ? su : sg; }, sa + row_of(32 * wn + (lane & 31)) * lds, 32 * wn >= n_at, acc);
     lds_barrier();          // (the buffers' last block is read)
     uint32_t *const most = reinterpret_cast<uint32_t *>(smem + PLACES * BLOCK);          // [2 waves][64 places], behind the tile's quantised rows
     const bool whole = n0 + BLOCK <= ff;
@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(64 * MoeTile::WAVES, 2) k_moe_fp8_down_tile(co
     const float *sd = sdown + ((size_t)e * wb + min(nw, width - 1) / BLOCK) * fb;
     tile_sums<WIDE, 1, true, T, 2>(
         smem, ff, down + ((size_t)e * width + n0) * ff, [&](int r) { return (uint32_t)min(r, width - 1 - n0) * (uint32_t)ff; }, q + (size_t)at0 * ff,
-        [&](int r) { return (uint32_t)min(r, n_at - 1) * (uint32_t)ff; }, [&](int) { return sd; }, s + (size_t)(at0 + min(32 * wn + (lane & 31), n_at - 1)) * fb, acc);
+        [&](int r) { return (uint32_t)min(r, n_at - 1) * (uint32_t)ff; }, [&](int) { return sd; }, s + (size_t)(at0 + min(32 * wn + (lane & 31), n_at - 1)) * fb, 32 * wn >= n_at || nw >= width, acc);
     tile_out<T, 4>(smem, acc, [&](int t, int n, float *v) {
         if (32 * wn + t < n_at && nw + n < width) *reinterpret_cast<u32x4 *>(out + (size_t)(at0 + 32 * wn + t) * width + nw + n) = pack<IFA_F32>(v);          // (width in whole 16s)
     });
