@@ -842,13 +842,14 @@ int ifa_moe_experts_routed_rows_f32(int score_kind, int renorm, float renorm_eps
 /* ======================================================================== */
 /* residual update, RMS norm and quantisation in one pass: x += m (m null: x as it is; the sum rounded to dtype), v = x / sqrt(mean(x^2) + eps) * (w_offset + w[c])
  * (w bf16 [cols], null: 0), (q, scale) = v quantised, h = v in dtype (nullable: what a router reads).  x, m and h [rows][ld*] of dtype, whole 16 bytes a row;
- * x, m and h are different buffers.  cols <= 32768. */
+ * x, m and h are different buffers.  cols <= 32768, rows < 2^22. */
 int ifa_norm_add_fp8(int dtype, void *x, size_t ldx, size_t rows, size_t cols, const void *m, size_t ldm, const void *w_bf16, float w_offset, float eps, void *h, size_t ldh,
                      void *q_e4m3, size_t ldq, void *scale_f32, size_t lds, ifa_stream stream);
 /* gated activation and quantisation: rows gate | up of 2 cols values, v = f(gate, up), kinds 0 / 1 / 2 / 3 as ifa_glu_ex_f32; kind 4: rows of cols values as they are */
 int ifa_glu_fp8(int kind, float limit, int dtype, const void *gate_up, size_t ld, size_t rows, size_t cols, void *q_e4m3, size_t ldq, void *scale_f32, size_t lds, ifa_stream stream);
 /* C[t][n] (+)= sum_b a_scale[t][b] w_scale[n / 128][b] (sum over block b of a[t][k] w[n][k]) + bias[n]; bias bf16 [rows] nullable; accumulate != 0 adds into C (the sum
- * rounded once to c_dtype).  Workspace: ifa_linear_fp8_workspace_bytes (a product without one, or with less, is the same but may be slower). */
+ * rounded once to c_dtype).  Products of a few hundred rows or less share their columns out to several workgroups through a workspace (16-byte aligned,
+ * ifa_linear_fp8_workspace_bytes; 0: it is not used); with less, or none, they take longer and add up in another order.  tokens <= 1000000, rows < 2^26. */
 size_t ifa_linear_fp8_workspace_bytes(size_t rows, size_t cols, size_t tokens);
 int ifa_linear_fp8(const void *w_e4m3, const void *w_scale_f32, size_t rows, size_t cols, const void *a_e4m3, size_t lda, const void *a_scale_f32, size_t lds, size_t tokens,
                    const void *bias_bf16, int accumulate, int c_dtype, void *c, size_t ldc, void *ws, size_t ws_bytes, ifa_stream stream);
@@ -861,7 +862,8 @@ int ifa_moe_route_groups_f32(int score_kind, int groups, int groups_kept, int gr
                              int top, const void *correction_f32, int *idx_dev, void *wgt_f32, ifa_stream stream);
 /* Gated experts over quantised rows: y[t] (+)= sum_k wgt[t][k] * Down_e q(f(Gate_e a[t], Up_e a[t])), e = idx[t][k], f as ifa_glu_fp8 (kinds 0 .. 3), q: quantised as above.  gate_up
  * [experts][gate ff | up ff][width] with scales [experts][2][ceil(ff / 128)][ceil(width / 128)], down [experts][width][ff] with scales [experts][ceil(width / 128)][ceil(ff / 128)].
- * idx outside 0 .. experts - 1 adds nothing; an expert may come more than once in a row.  width and ff in whole 16s. */
+ * idx outside 0 .. experts - 1 adds nothing; an expert may come more than once in a row.  width and ff in whole 16s; experts <= 1024, top <= 64, rows * top <= 1000000,
+ * 2 ff width < 2^32.  idx_dev is read by more than one launch: it stays as it is until the call's work is done. */
 size_t ifa_moe_experts_fp8_workspace_bytes(size_t rows, int top, int width, int ff, int experts);
 int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t lda, const void *a_scale_f32, size_t lds, size_t rows, int width, int ff, int experts, int top,
                         const void *gate_up_e4m3, const void *gate_up_scale_f32, const void *down_e4m3, const void *down_scale_f32, const int *idx_dev, const void *wgt_f32, void *ws,

@@ -136,7 +136,7 @@ int ifa_norm_add_fp8(int dtype, void *x, size_t ldx, size_t rows, size_t cols, c
     IFA_REQUIRE(x && q_e4m3 && scale_f32, "ifa_norm_add_fp8: null pointer");
     if (!elem_known(dtype)) return ifa_fail(IFA_ERR_DTYPE, "ifa_norm_add_fp8: dtype %d (F32, F16 or BF16)", dtype);
     const size_t n = 16 / elem_bytes(dtype);
-    IFA_REQUIRE(rows > 0 && rows < (1u << 31) && cols > 0 && cols % 16 == 0 && cols <= 32768, "ifa_norm_add_fp8: %zu rows of %zu columns (whole 16s up to 32768)", rows, cols);
+    IFA_REQUIRE(rows > 0 && rows < (1u << 22) && cols > 0 && cols % 16 == 0 && cols <= 32768, "ifa_norm_add_fp8: %zu rows (fewer than 2^22) of %zu columns (whole 16s up to 32768)", rows, cols);
     IFA_REQUIRE(ldx >= cols && ldx % n == 0 && (!m || (ldm >= cols && ldm % n == 0)) && (!h || (ldh >= cols && ldh % n == 0)) && ldq >= cols && ldq % 16 == 0 && lds >= blocks_of(cols),
                 "ifa_norm_add_fp8: row strides (rows of whole 16 bytes)");
     IFA_REQUIRE(aligned16(x) && aligned16(m) && aligned16(h) && aligned16(q_e4m3) && ((uintptr_t)w_bf16 & 1) == 0 && ((uintptr_t)scale_f32 & 3) == 0, "ifa_norm_add_fp8: misaligned pointer");
@@ -151,7 +151,7 @@ int ifa_glu_fp8(int kind, float limit, int dtype, const void *gate_up, size_t ld
     if (!elem_known(dtype)) return ifa_fail(IFA_ERR_DTYPE, "ifa_glu_fp8: dtype %d (F32, F16 or BF16)", dtype);
     const size_t n = 16 / elem_bytes(dtype);
     IFA_REQUIRE(kind >= 0 && kind <= 4, "ifa_glu_fp8: kind %d", kind);
-    IFA_REQUIRE(rows > 0 && cols > 0 && cols % 16 == 0 && cols < (1u << 30) && rows * (blocks_of(cols) * BLOCK / n) < ((size_t)1 << 38), "ifa_glu_fp8: %zu rows of %zu columns (whole 16s)", rows, cols);
+    IFA_REQUIRE(rows > 0 && cols > 0 && cols % 16 == 0 && cols < (1u << 30) && rows < (1u << 31) && rows * (blocks_of(cols) * BLOCK / n) < 0xFFFFFF00u, "ifa_glu_fp8: %zu rows of %zu columns (whole 16s, fewer than 2^32 pieces of 16 bytes)", rows, cols);
     IFA_REQUIRE(ld >= cols * (kind == 4 ? 1 : 2) && ld % n == 0 && ldq >= cols && ldq % 16 == 0 && lds >= blocks_of(cols), "ifa_glu_fp8: row strides (rows of whole 16 bytes)");
     IFA_REQUIRE(aligned16(gate_up) && aligned16(q_e4m3) && ((uintptr_t)scale_f32 & 3) == 0, "ifa_glu_fp8: misaligned pointer");
     auto f = dtype == IFA_F32 ? glu<IFA_F32> : dtype == IFA_F16 ? glu<IFA_F16> : glu<IFA_BF16>;

@@ -230,7 +230,7 @@ extern "C" {
 
 size_t ifa_linear_fp8_workspace_bytes(size_t rows, size_t cols, size_t tokens) 
 {
-    if (rows == 0 || cols == 0 || tokens == 0 || rows >= (1u << 30) || cols >= (1u << 30) || tokens > 1000000) return 0;
+    if (rows == 0 || cols == 0 || tokens == 0 || rows >= (1u << 26) || cols >= (1u << 30) || tokens > 1000000) return 0;
     size_t most = 0;
     for (int wide = 0; wide < 2; wide++) {
         const Plan plan = choose(wide, rows, cols, tokens, (size_t)256 << 20);
@@ -244,7 +244,7 @@ int ifa_linear_fp8(const void *w_e4m3, const void *w_scale_f32, size_t rows, siz
 {
     IFA_REQUIRE(w_e4m3 && w_scale_f32 && a_e4m3 && a_scale_f32 && c, "ifa_linear_fp8: null pointer");
     if (!elem_known(c_dtype)) return ifa_fail(IFA_ERR_DTYPE, "ifa_linear_fp8: output dtype %d (F32, F16 or BF16)", c_dtype);
-    IFA_REQUIRE(rows > 0 && cols > 0 && tokens > 0 && cols % 16 == 0 && rows < (1u << 30) && cols < (1u << 30) && tokens <= 1000000, "ifa_linear_fp8: %zu x %zu over %zu rows (columns in whole 16s)", rows,
+    IFA_REQUIRE(rows > 0 && cols > 0 && tokens > 0 && cols % 16 == 0 && rows < (1u << 26) && cols < (1u << 30) && tokens <= 1000000, "ifa_linear_fp8: %zu x %zu over %zu rows (columns in whole 16s)", rows,
                 cols, tokens);
     IFA_REQUIRE(lda >= cols && lda % 16 == 0 && lds >= blocks_of(cols) && ldc >= rows, "ifa_linear_fp8: row strides");
     IFA_REQUIRE((((uintptr_t)w_e4m3 | (uintptr_t)a_e4m3 | (uintptr_t)ws) & 15) == 0 && (((uintptr_t)w_scale_f32 | (uintptr_t)a_scale_f32) & 3) == 0 && ((uintptr_t)bias_bf16 & 1) == 0

@@ -609,7 +609,7 @@ int ifa_moe_route_groups_f32(int score_kind, int groups, int groups_kept, int gr
 {
     IFA_REQUIRE(logits_f32 && idx_dev && wgt_f32, "ifa_moe_route_groups_f32: null pointer");
     IFA_REQUIRE(score_kind == 0 || score_kind == 1, "ifa_moe_route_groups_f32: score kind %d", score_kind);
-    IFA_REQUIRE(rows > 0 && rows < (1u << 31) && n_all > 0 && n_all <= 1024 && ld >= (size_t)n_all, "ifa_moe_route_groups_f32: %zu rows of %d experts (1024 at most)", rows, n_all);
+    IFA_REQUIRE(rows > 0 && rows < (1u << 25) && n_all > 0 && n_all <= 1024 && ld >= (size_t)n_all, "ifa_moe_route_groups_f32: %zu rows (fewer than 2^25) of %d experts (1024 at most)", rows, n_all);
     IFA_REQUIRE(groups > 0 && groups <= 64 && n_all % groups == 0 && groups_kept > 0 && groups_kept <= groups && (group_best == 1 || group_best == 2),
                 "ifa_moe_route_groups_f32: %d of %d groups by their best %d", groups_kept, groups, group_best);
     IFA_REQUIRE(top > 0 && top <= 64 && top <= groups_kept * (n_all / groups), "ifa_moe_route_groups_f32: %d of %d experts", top, groups_kept * (n_all / groups));
@@ -635,7 +635,7 @@ int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t ld
     if (!elem_known(y_dtype)) return ifa_fail(IFA_ERR_DTYPE, "ifa_moe_experts_fp8: output dtype %d (F32, F16 or BF16)", y_dtype);
     IFA_REQUIRE(glu_kind >= 0 && glu_kind <= 3, "ifa_moe_experts_fp8: activation %d", glu_kind);
     IFA_REQUIRE(rows > 0 && width > 0 && ff > 0 && width % 16 == 0 && ff % 16 == 0 && experts > 0 && experts <= 1024 && top > 0 && top <= 64 && rows * top <= 1000000 && width <= 65536 && ff <= 65536
-                    && 2 * (size_t)ff * width < (1ull << 32),
+                    && 2 * (size_t)ff * width < (1ull << 32) && rows * ((size_t)width / 4) < 0xFFFFFF00u,
                 "ifa_moe_experts_fp8: %zu rows x %d of %d experts, %d x %d (whole 16s)", rows, top, experts, width, ff);
     IFA_REQUIRE(lda >= (size_t)width && lda % 16 == 0 && lds >= blocks_of(width) && ldy >= (size_t)width, "ifa_moe_experts_fp8: row strides");
     IFA_REQUIRE((((uintptr_t)a_e4m3 | (uintptr_t)gate_up_e4m3 | (uintptr_t)down_e4m3 | (uintptr_t)ws) & 15) == 0 && (((uintptr_t)a_scale_f32 | (uintptr_t)gate_up_scale_f32 | (uintptr_t)down_scale_f32) & 3) == 0

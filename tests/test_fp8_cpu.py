@@ -29,32 +29,32 @@ EXPERTS = dict(kind=0, limit=7.0, a=P, lda=64, sa=P, lds=1, rows=3, width=64, ff
 
 @pytest.mark.parametrize("changed", [dict(x=None), dict(q=None), dict(scale=None), dict(rows=0), dict(cols=0), dict(cols=40), dict(cols=32768 + 16, ldx=40000, ldm=40000, ldh=40000, ldq=40000, lds=300),
                                      dict(ldx=48), dict(ldx=66), dict(ldm=48), dict(ldh=48), dict(ldq=56), dict(ldq=72), dict(lds=0), dict(x=P + 4), dict(m=P + 8), dict(h=P + 4), dict(q=P + 8),
-                                     dict(w=P + 1), dict(scale=P + 2), dict(h=P), dict(m=P)])
+                                     dict(w=P + 1), dict(scale=P + 2), dict(h=P), dict(m=P), dict(rows=1 << 22)])
 def test_norm_refuses(changed):
     assert call("ifa_norm_add_fp8", NORM, **changed) == ARG and b"ifa_norm_add_fp8" in ia.lib().ifa_last_error()
 
 
 @pytest.mark.parametrize("changed", [dict(gu=None), dict(q=None), dict(scale=None), dict(kind=-1), dict(kind=5), dict(rows=0), dict(cols=8), dict(ld=64), dict(ld=132), dict(ldq=48), dict(lds=0),
-                                     dict(gu=P + 2), dict(q=P + 4)])
+                                     dict(gu=P + 2), dict(q=P + 4), dict(rows=1 << 30)])
 def test_activation_refuses(changed):
     assert call("ifa_glu_fp8", GLU, **changed) == ARG and b"ifa_glu_fp8" in ia.lib().ifa_last_error()
 
 
 @pytest.mark.parametrize("changed", [dict(w=None), dict(sw=None), dict(a=None), dict(sa=None), dict(c=None), dict(rows=0), dict(tokens=0), dict(cols=0), dict(cols=136), dict(lda=128), dict(lda=152),
-                                     dict(lds=1), dict(ldc=31), dict(w=P + 8), dict(a=P + 4), dict(c=P + 1), dict(bias=P + 1), dict(sa=P + 2), dict(tokens=1000001), dict(rows=1 << 30)])
+                                     dict(lds=1), dict(ldc=31), dict(w=P + 8), dict(a=P + 4), dict(c=P + 1), dict(bias=P + 1), dict(sa=P + 2), dict(tokens=1000001), dict(rows=1 << 26, ldc=1 << 26)])
 def test_product_refuses(changed):
     assert call("ifa_linear_fp8", LINEAR, **changed) == ARG and b"ifa_linear_fp8" in ia.lib().ifa_last_error()
 
 
 @pytest.mark.parametrize("changed", [dict(logits=None), dict(idx=None), dict(wgt=None), dict(score=2), dict(groups=0), dict(groups=5), dict(groups=65, n_all=130, ld=130), dict(kept=0), dict(kept=5),
-                                     dict(best=0), dict(best=3), dict(top=0), dict(top=17), dict(kept=4, groups=4, n_all=512, ld=512, top=65), dict(n_all=1028, ld=1028), dict(ld=31), dict(rows=0)])
+                                     dict(best=0), dict(best=3), dict(top=0), dict(top=17), dict(kept=4, groups=4, n_all=512, ld=512, top=65), dict(n_all=1028, ld=1028), dict(ld=31), dict(rows=0), dict(rows=1 << 25)])
 def test_router_refuses(changed):
     assert call("ifa_moe_route_groups_f32", ROUTE, **changed) == ARG and b"ifa_moe_route_groups_f32" in ia.lib().ifa_last_error()
 
 
 @pytest.mark.parametrize("changed", [dict(a=None), dict(sa=None), dict(gu=None), dict(sgu=None), dict(down=None), dict(sdown=None), dict(idx=None), dict(wgt=None), dict(ws=None), dict(y=None),
                                      dict(kind=4), dict(kind=-1), dict(rows=0), dict(width=72), dict(ff=40), dict(experts=0), dict(experts=1025), dict(top=0), dict(top=65), dict(lda=48), dict(lda=72),
-                                     dict(lds=0), dict(ldy=63), dict(ws_bytes=100), dict(ws=P + 8), dict(gu=P + 8), dict(down=P + 1), dict(y=P + 2), dict(rows=600000)])
+                                     dict(lds=0), dict(ldy=63), dict(ws_bytes=100), dict(ws=P + 8), dict(gu=P + 8), dict(down=P + 1), dict(y=P + 2), dict(rows=600000), dict(width=65536, ff=32768, lda=65536, lds=512, ldy=65536), dict(width=65536, ff=16, lda=65536, lds=512, ldy=65536, rows=300000)])
 def test_experts_refuse(changed):
     assert call("ifa_moe_experts_fp8", EXPERTS, **changed) == ARG and b"ifa_moe_experts_fp8" in ia.lib().ifa_last_error()
 
