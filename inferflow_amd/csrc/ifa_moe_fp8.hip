@@ -649,7 +649,10 @@ int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t ld
     uint8_t *q = base + W.q;
     const hipStream_t st = ifa_s(stream);
     const size_t few_lds = (size_t)2 * ((top + 1) / 2) * blocks_of(ff) * (BLOCK + 4);
-    if (rows <= 4 && few_lds <= 48 * 1024) {
+    // one or two rows, or up to four of small matrices: a stream for each pair.  us pairs / lists, rows x choices of experts, width x ff: 1 x 6 of 64, 2048 x 1408 20.6 / 33.5, 2 28.1 / 37.6, 4 48.4 / 47.8;
+    // 4 x 4 of 16, 1024 x 704 14.9 / 17.2, 8 25.5 / 18.4; 2 x 2 of 8, 4096 x 4096 54 / 55, 3 76 / 64
+    const double bytes = 3.0 * width * ff;
+    if ((rows <= 2 || (rows <= 4 && bytes <= 4e6)) && few_lds <= 48 * 1024) {
         hipLaunchKernelGGL(k_moe_fp8_up_pairs, dim3(ff / 16, pairs), dim3(64 * PAIR_WAVES), 0, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, experts, top,
                            (const uint8_t *)a_e4m3, lda, (const float *)a_scale_f32, lds, idx_dev, glu_kind, limit, act);
 #define IFA_DOWN(DT) hipLaunchKernelGGL((k_moe_fp8_down_pairs<DT, 3>), dim3(width / 8, (unsigned)rows), dim3(64 * PAIR_WAVES), few_lds, st, (const uint8_t *)down_e4m3, (const float *)down_scale_f32, \
@@ -659,7 +662,9 @@ int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t ld
         IFA_LAUNCH_CHECK();
         return IFA_OK;
     }
-    const bool wide = y_dtype == IFA_F32, many = pairs > LIST_MAX || pairs / experts >= 16 || ff > DOWN_FF;
+    // lists go through an expert's matrices once for each 32 of its rows, tiles once for each 128 but with four launches more about them.  us lists / tiles, rows: 64 experts of 2048 x 1408, top 6,
+    // 64 126 / 141, 100 145 / 135, 256 235 / 145; 32 of 2048 x 704, top 4, 96 47 / 50, 160 58 / 51; 16 of 1024 x 704, top 4, 64 27 / 39, 128 39 / 40, 256 60 / 41; 8 of 4096 x 4096, top 2, 48 110 / 121, 64 135 / 120
+    const bool wide = y_dtype == IFA_F32, many = pairs > LIST_MAX || ff > DOWN_FF || (double)pairs / experts >= (experts * bytes > 256e6 ? 12.0 : experts * bytes > 64e6 ? 15.0 : 30.0);
     if (many) {
         const int max_tiles = pairs / PLACES + std::min(pairs, experts);
         const size_t g_up = blocks_of(ff) * max_tiles, g_down = (size_t)((width + 255) / 256) * max_tiles;
