@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(256) k_glu_fp8(int kind, float limit, const ty
             float u[N];
             unpack<DT>(*reinterpret_cast<const u32x4 *>(gu + t * ld + cols + c), u);
 #pragma unroll
-            for (int e = 0; e < N; e++) v[e] = ifa32::glu_of(kind, limit, v[e], u[e]);
+            for (int e = 0; e < N; e++) v[e] = gated(kind, limit, v[e], u[e]);
         }
 #pragma unroll
         for (int e = 0; e < N; e++) most = dpp_max(most, abs_bits(v[e]));

@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(64 * PAIR_WAVES) k_moe_fp8_up_pairs(const uint
     if (wave > 0 || (lane & 15)) return;          // (the sixteen activation rows of the products are one and the same)
     f32x4 v;
 #pragma unroll
-    for (int r = 0; r < 4; r++) v[r] = ifa32::glu_of(kind, limit, acc[0][0][r], acc[1][0][r]);
+    for (int r = 0; r < 4; r++) v[r] = gated(kind, limit, acc[0][0][r], acc[1][0][r]);
     *reinterpret_cast<f32x4 *>(act + (size_t)p * ff + n0 + 4 * (lane >> 4)) = v;
 }
 
@@ -311,7 +311,7 @@ __device__ __forceinline__ void up_list(const uint16_t *list, int n, const uint8
             if (16 * j + i >= n) continue;
             f32x4 v;
 #pragma unroll
-            for (int r = 0; r < 4; r++) v[r] = ifa32::glu_of(kind, limit, acc[0][j][r], acc[1][j][r]);
+            for (int r = 0; r < 4; r++) v[r] = gated(kind, limit, acc[0][j][r], acc[1][j][r]);
             *reinterpret_cast<f32x4 *>(act + (size_t)list[16 * j + i] * ff + n0 + 4 * (lane >> 4)) = v;
         }
     }
@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(64 * MoeTile::WAVES, 2) k_moe_fp8_up_tile(cons
         for (int m = 0; m < 4; m++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                float v = ifa32::glu_of(kind, limit, acc[m][j][r], acc[m + 4][j][r]);
+                float v = gated(kind, limit, acc[m][j][r], acc[m + 4][j][r]);
                 if (!whole && n0 + 64 * wm + 16 * m >= ff) v = 0.0f;          // (ff in whole 16s)
                 acc[m][j][r] = v;
                 mine[j] = dpp_max(mine[j], abs_bits(v));
