@@ -845,7 +845,8 @@ int ifa_moe_experts_routed_rows_f32(int score_kind, int renorm, float renorm_eps
  * x, m and h are different buffers.  cols <= 32768, rows < 2^22. */
 int ifa_norm_add_fp8(int dtype, void *x, size_t ldx, size_t rows, size_t cols, const void *m, size_t ldm, const void *w_bf16, float w_offset, float eps, void *h, size_t ldh,
                      void *q_e4m3, size_t ldq, void *scale_f32, size_t lds, ifa_stream stream);
-/* gated activation and quantisation: rows gate | up of 2 cols values, v = f(gate, up), kinds 0 / 1 / 2 / 3 as ifa_glu_ex_f32; kind 4: rows of cols values as they are */
+/* gated activation and quantisation: rows gate | up of 2 cols values, v = f(gate, up), kinds 0 / 1 / 2 / 3 as ifa_glu_ex_f32 (but a NaN stays one, and a sigmoid below
+ * 2^-127 is 0); kind 4: rows of cols values as they are.  Fewer than 2^32 pieces of 16 bytes */
 int ifa_glu_fp8(int kind, float limit, int dtype, const void *gate_up, size_t ld, size_t rows, size_t cols, void *q_e4m3, size_t ldq, void *scale_f32, size_t lds, ifa_stream stream);
 /* C[t][n] (+)= sum_b a_scale[t][b] w_scale[n / 128][b] (sum over block b of a[t][k] w[n][k]) + bias[n]; bias bf16 [rows] nullable; accumulate != 0 adds into C (the sum
  * rounded once to c_dtype).  Products of a few hundred rows or less share their columns out to several workgroups through a workspace (16-byte aligned,
@@ -863,7 +864,7 @@ int ifa_moe_route_groups_f32(int score_kind, int groups, int groups_kept, int gr
 /* Gated experts over quantised rows: y[t] (+)= sum_k wgt[t][k] * Down_e q(f(Gate_e a[t], Up_e a[t])), e = idx[t][k], f as ifa_glu_fp8 (kinds 0 .. 3), q: quantised as above.  gate_up
  * [experts][gate ff | up ff][width] with scales [experts][2][ceil(ff / 128)][ceil(width / 128)], down [experts][width][ff] with scales [experts][ceil(width / 128)][ceil(ff / 128)].
  * idx outside 0 .. experts - 1 adds nothing; an expert may come more than once in a row.  width and ff in whole 16s; experts <= 1024, top <= 64, rows * top <= 1000000,
- * 2 ff width < 2^32.  idx_dev is read by more than one launch: it stays as it is until the call's work is done. */
+ * 2 ff width < 2^32 (the workspace of sizes beyond these: 0 bytes, and the call is refused).  idx_dev is read by more than one launch: it stays as it is until the call's work is done. */
 size_t ifa_moe_experts_fp8_workspace_bytes(size_t rows, int top, int width, int ff, int experts);
 int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t lda, const void *a_scale_f32, size_t lds, size_t rows, int width, int ff, int experts, int top,
                         const void *gate_up_e4m3, const void *gate_up_scale_f32, const void *down_e4m3, const void *down_scale_f32, const int *idx_dev, const void *wgt_f32, void *ws,

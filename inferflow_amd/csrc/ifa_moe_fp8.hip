@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(1024) k_moe_fp8_place(const int *__restrict__ 
     }
 }
 
-// Tiles of 64 places of one expert.  A workgroup of four waves, two a compute unit.
+// Tiles of 128 places of one expert.  A workgroup of eight waves, one a compute unit.
 constexpr int PLACES = 128;
 typedef Tile<256, PLACES, 2, PLACES / 32> MoeTile;
 
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(64 * MoeTile::WAVES, 2) k_moe_fp8_up_tile(cons
         smem, width, gu + (size_t)e * 2 * ff * width, [&](int r) { return (uint32_t)((r < BLOCK ? 0 : ff) + min(n0 + (r & (BLOCK - 1)), ff - 1)) * (uint32_t)width; }, nullptr,
         [&](int r) { return a + row_of(r) * lda; }, [&](int h) { return h ? su : sg; }, sa + row_of(32 * wn + (lane & 31)) * lds, 32 * wn >= n_at, acc);
     lds_barrier();          // (the buffers' last block is read)
-    uint32_t *const most = reinterpret_cast<uint32_t *>(smem + PLACES * BLOCK);          // [2 waves][64 places], behind the tile's quantised rows
+    uint32_t *const most = reinterpret_cast<uint32_t *>(smem + PLACES * BLOCK);          // [2 waves][PLACES], behind the tile's quantised rows
     const bool whole = n0 + BLOCK <= ff;
     uint32_t mine[T::TN];
 #pragma unroll
@@ -612,6 +612,13 @@ struct Work {
     }
 };
 
+// what fits the kernels' 32-bit offsets, lists and grids
+bool sizes_known(size_t rows, int top, int width, int ff, int experts)
+{
+    return rows > 0 && rows <= 1000000 && top > 0 && top <= 64 && rows * top <= 1000000 && width > 0 && width <= 65536 && width % 16 == 0 && ff > 0 && ff <= 65536 && ff % 16 == 0 && experts > 0
+           && experts <= 1024 && 2 * (size_t)ff * width < (1ull << 32) && rows * ((size_t)width / 4) < 0xFFFFFF00u;
+}
+
 } // namespace
 
 extern "C" {
@@ -635,7 +642,7 @@ int ifa_moe_route_groups_f32(int score_kind, int groups, int groups_kept, int gr
 
 size_t ifa_moe_experts_fp8_workspace_bytes(size_t rows, int top, int width, int ff, int experts)
 {
-    if (rows == 0 || rows > (1u << 24) || top <= 0 || width <= 0 || ff <= 0 || experts <= 0) return 0;
+    if (!sizes_known(rows, top, width, ff, experts)) return 0;
     return Work(rows, top, width, ff, experts).bytes;
 }
 
@@ -646,8 +653,7 @@ int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t ld
     IFA_REQUIRE(a_e4m3 && a_scale_f32 && gate_up_e4m3 && gate_up_scale_f32 && down_e4m3 && down_scale_f32 && idx_dev && wgt_f32 && ws && y, "ifa_moe_experts_fp8: null pointer");
     if (!elem_known(y_dtype)) return ifa_fail(IFA_ERR_DTYPE, "ifa_moe_experts_fp8: output dtype %d (F32, F16 or BF16)", y_dtype);
     IFA_REQUIRE(glu_kind >= 0 && glu_kind <= 3, "ifa_moe_experts_fp8: activation %d", glu_kind);
-    IFA_REQUIRE(rows > 0 && width > 0 && ff > 0 && width % 16 == 0 && ff % 16 == 0 && experts > 0 && experts <= 1024 && top > 0 && top <= 64 && rows * top <= 1000000 && width <= 65536 && ff <= 65536
-                    && 2 * (size_t)ff * width < (1ull << 32) && rows * ((size_t)width / 4) < 0xFFFFFF00u,
+    IFA_REQUIRE(sizes_known(rows, top, width, ff, experts),
                 "ifa_moe_experts_fp8: %zu rows x %d of %d experts, %d x %d (whole 16s)", rows, top, experts, width, ff);
     IFA_REQUIRE(lda >= (size_t)width && lda % 16 == 0 && lds >= blocks_of(width) && ldy >= (size_t)width, "ifa_moe_experts_fp8: row strides");
     IFA_REQUIRE((((uintptr_t)a_e4m3 | (uintptr_t)gate_up_e4m3 | (uintptr_t)down_e4m3 | (uintptr_t)ws) & 15) == 0 && (((uintptr_t)a_scale_f32 | (uintptr_t)gate_up_scale_f32 | (uintptr_t)down_scale_f32) & 3) == 0

@@ -71,6 +71,14 @@ def test_workspaces_grow_with_the_work():
     assert f(0, 2, 64, 48, 4) == f(1, 0, 64, 48, 4) == f(1, 2, -64, 48, 4) == 0
 
 
+@pytest.mark.parametrize("sizes", [(1000001, 1, 64, 48, 4), (600000, 2, 64, 48, 4), (1 << 62, 4, 64, 48, 4), (1, 65, 64, 48, 4), (1, 2, 72, 48, 4), (1, 2, 64, 40, 4), (1, 2, 65552, 48, 4),
+                                   (1, 2, 64, 65552, 4), (1, 2, 64, 48, 1025), (1, 2, 65536, 32768, 4), (300000, 2, 65536, 16, 4)])
+def test_sizes_that_are_refused_have_no_workspace(sizes):
+    rows, top, width, ff, E = sizes
+    assert ia.lib().ifa_moe_experts_fp8_workspace_bytes(*sizes) == 0
+    assert call("ifa_moe_experts_fp8", EXPERTS, rows=rows, top=top, width=width, ff=ff, experts=E, lda=width, lds=orc.blocks(width), ldy=width, ws_bytes=1 << 60) == ARG
+
+
 def test_oracle_rounds_to_e4m3_like_torch():
     v = torch.cat([torch.linspace(-460, 460, 20001, dtype=torch.float64), torch.linspace(-0.07, 0.07, 20001, dtype=torch.float64)])
     every = torch.arange(256, dtype=torch.uint8).view(orc.F8).double()

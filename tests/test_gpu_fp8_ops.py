@@ -131,6 +131,46 @@ def test_activation(dtype, kind, rows, cols):
     assert (q[:, cols:] == 0x55).all() and (scale[:, -1] == 3.0).all()
 
 
+@pytest.mark.parametrize("kind", [0, 1, 2, 3])
+def test_activation_of_small_and_large_gates(kind):
+    """one gate a block, so that its scale is the activation's size over 448"""
+    one = torch.cat([torch.tensor([0.0, 1e-30, 1e-6, 0.3, 1.0, 6.9, 7.1, 15.0, 40.0, 87.0, 88.5, 89.0, 100.0, 1e4, 1e18, 3e38]), torch.linspace(0.01, 87.0, 200)])
+    a = torch.cat([one, -one])
+    n = len(a)
+    gu = torch.zeros(1, 2 * n * 128, device="cuda")
+    gu[0, :n * 128:128] = a.cuda()
+    gu[0, n * 128::128] = 1.0
+    q, scale = codes(1, n * 128), torch.zeros(1, n, device="cuda")
+    glu(kind, 0, gu, n * 128, q, scale); sync()
+    d, factor = a.double(), 1.0
+    if kind == 3:
+        d, factor = d.clamp_max(7.0), 2.0
+    x = {0: d, 1: 2 * math.sqrt(2 / math.pi) * (d + 0.044715 * d ** 3), 2: d, 3: 1.702 * d}[kind]
+    want = d.clamp_min(0) if kind == 2 else d * torch.sigmoid(x) * factor
+    # In steps of 2^-24: the power of two and the reciprocal 2 each, five roundings beside them, the scale's quotient 1; the exponent's argument is three roundings off, and x times that is in the power.
+    rel = torch.full_like(d, 1.0) if kind == 2 else 10 + 4 * x.abs().clamp_max(90)
+    # (where the sigmoid is below 2^-126 it may be 0)
+    lost = torch.where(x < -87, d.abs() * factor * 2.0 ** -125, 0.0)
+    got = scale[0].cpu().double() * 448
+    want = want.abs().clamp_min(448 * orc.TINY)
+    assert ((got - want).abs() <= 2.0 ** -24 * rel * want + lost).all()
+    v = q[0, ::128].view(F8).double().cpu()
+    assert torch.equal(v[want > 450 * orc.TINY].abs(), torch.full_like(v[want > 450 * orc.TINY], 448.0))
+
+
+@pytest.mark.parametrize("kind", [0, 1, 2, 3])
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_a_gate_or_factor_that_is_no_number_stays_none(kind, dtype):
+    gu = torch.ones(4, 512, device="cuda", dtype=TYPES[dtype])
+    gu[0, 5], gu[1, 261], gu[2, 5] = math.nan, math.nan, math.inf
+    q, scale = codes(4, 256), torch.zeros(4, 2, device="cuda")
+    glu(kind, dtype, gu, 256, q, scale); sync()
+    back = q.view(F8).double() * orc.per_column(scale, 256)
+    for t in (0, 1):
+        assert back[t, :128].isnan().all() and torch.isfinite(back[t, 128:]).all()
+    assert torch.isfinite(back[3]).all() and (kind == 3 or back[2, :128].isnan().all())          # (kind 3 clamps an infinite gate)
+
+
 def test_blocks_of_zeros_of_tiny_and_of_huge_values():
     v = torch.zeros(4, 384, device="cuda")
     v[1] = 1e-44; v[1, 130] = 1e-39
