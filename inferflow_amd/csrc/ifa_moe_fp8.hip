@@ -3,6 +3,7 @@
 //            the largest values the `top` largest choices are taken (the lower index wins a tie everywhere); weight = score [/ (sum of the taken + eps)] * scale
 //   experts  y[t] (+)= sum_k wgt[t][k] * Down_e q(act(Gate_e a[t]) * (Up_e a[t])),  e = idx[t][k];  q: rows in e4m3 with a scale for each 128 columns
 #include <algorithm>
+#include <cmath>
 #include "ifa_host.h"
 #include "ifa_fp8_stream.h"
 #include "ifa_fp8_tile.h"
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__(64 * DOWN_WAVES) k_moe_fp8_down_list(const uin
 }
 
 // ---- many rows: the pairs sorted by expert.  k_moe_fp8_count leaves, for each block of `per` pairs, how many of them chose each expert; k_moe_fp8_place adds these counts up and gives the pairs
-// their places: place_row[at] = the row of the pair at sorted place `at`, pair_at[p] = the place of pair p (-1: none), tiles = {expert, first place, places} of at most PLACES places of one
+// their places: place_row[at] = the row of the pair at sorted place `at`, pair_at[p] = the place of pair p (-1: none), tiles = {expert, first place, places} of at most `tile` places of one
 // expert, *n_tiles.  (A workgroup alone took 31 us for 18000 pairs.)  A pair's place within its block's part of an expert's range is a matter of order alone: no value depends on it.
 __global__ void __launch_bounds__(1024) k_moe_fp8_count(const int *__restrict__ idx, int pairs, int experts, int per, int *__restrict__ counts)
 {
@@ -460,9 +461,8 @@ __global__ void __launch_bounds__(1024) k_moe_fp8_place(const int *__restrict__ 
     }
 }
 
-// Tiles of 128 places of one expert.  A workgroup of eight waves, one a compute unit.
-constexpr int PLACES = 128;
-typedef Tile<256, PLACES, 2, PLACES / 32> MoeTile;
+// Tiles of 128, 192 or 256 places of one expert (places_for).  A workgroup of eight waves, one a compute unit.
+template <int PLACES> using MoeTile = Tile<256, PLACES, 2, 4>;
 
 // the tile's place among those that there are (the empty ones behind them are dealt to nobody); tiles of one expert side by side
 __device__ __forceinline__ bool moe_tile(const int *n_tiles, int blocks, int &tile, int &block)
@@ -477,11 +477,13 @@ __device__ __forceinline__ bool moe_tile(const int *n_tiles, int blocks, int &ti
 }
 
 // a tile of 128 gate rows and the 128 up rows of the same columns: one block of the activations, which leave it quantised
-__global__ void __launch_bounds__(64 * MoeTile::WAVES, 2) k_moe_fp8_up_tile(const uint8_t *__restrict__ gu, const float *__restrict__ sgu, int width, int ff, const uint8_t *__restrict__ a, size_t lda,
+template <int PLACES>
+__global__ void __launch_bounds__(512, 2) k_moe_fp8_up_tile(const uint8_t *__restrict__ gu, const float *__restrict__ sgu, int width, int ff, const uint8_t *__restrict__ a, size_t lda,
                                                             const float *__restrict__ sa, size_t lds, const int *__restrict__ place_row, const int *__restrict__ tiles,
                                                             const int *__restrict__ n_tiles, int kind, float limit, uint8_t *__restrict__ q, float *__restrict__ s)
 {
-    typedef MoeTile T;
+    typedef MoeTile<PLACES> T;
+    constexpr int MINE = 16 * T::TN;          // places of a wave
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1, g = lane >> 4, i = lane & 15, fb = (int)blocks_of(ff);
     int tile, block;
@@ -497,7 +499,7 @@ __global__ void __launch_bounds__(64 * MoeTile::WAVES, 2) k_moe_fp8_up_tile(cons
     auto row_of = [&](int r) { return (size_t)place_row[at0 + min(r, n_at - 1)]; };
     tile_sums<false, 2, false, T, 2>(
         smem, width, gu + (size_t)e * 2 * ff * width, [&](int r) { return (uint32_t)((r < BLOCK ? 0 : ff) + min(n0 + (r & (BLOCK - 1)), ff - 1)) * (uint32_t)width; }, nullptr,
-        [&](int r) { return a + row_of(r) * lda; }, [&](int h) { return h ? su : sg; }, sa + row_of(32 * wn + (lane & 31)) * lds, 32 * wn >= n_at, acc);
+        [&](int r) { return a + row_of(r) * lda; }, [&](int h) { return h ? su : sg; }, sa + row_of(MINE * wn + lane % MINE) * lds, MINE * wn >= n_at, acc);
     lds_barrier();          // (the buffers' last block is read)
     uint32_t *const most = reinterpret_cast<uint32_t *>(smem + PLACES * BLOCK);          // [2 waves][PLACES], behind the tile's quantised rows
     const bool whole = n0 + BLOCK <= ff;
@@ -516,12 +518,12 @@ __global__ void __launch_bounds__(64 * MoeTile::WAVES, 2) k_moe_fp8_up_tile(cons
             }
         mine[j] = dpp_max(mine[j], (uint32_t)__shfl_xor((int)mine[j], 16, 64));
         mine[j] = dpp_max(mine[j], (uint32_t)__shfl_xor((int)mine[j], 32, 64));
-        if (g == 0) most[wm * PLACES + 32 * wn + 16 * j + i] = mine[j];
+        if (g == 0) most[wm * PLACES + MINE * wn + 16 * j + i] = mine[j];
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < T::TN; j++) {
-        const int at = 32 * wn + 16 * j + i;
+        const int at = MINE * wn + 16 * j + i;
         const float sc = scale_of(dpp_max(most[at], most[PLACES + at])), inv = 1.0f / sc;
         if (wm == 0 && g == 0 && at < n_at) s[(size_t)(at0 + at) * fb + block] = sc;
 #pragma unroll
@@ -538,11 +540,12 @@ __global__ void __launch_bounds__(64 * MoeTile::WAVES, 2) k_moe_fp8_up_tile(cons
     }
 }
 
-template <bool WIDE>
-__global__ void __launch_bounds__(64 * MoeTile::WAVES, 2) k_moe_fp8_down_tile(const uint8_t *__restrict__ down, const float *__restrict__ sdown, int width, int ff, const uint8_t *__restrict__ q,
+template <bool WIDE, int PLACES>
+__global__ void __launch_bounds__(512, 2) k_moe_fp8_down_tile(const uint8_t *__restrict__ down, const float *__restrict__ sdown, int width, int ff, const uint8_t *__restrict__ q,
                                                               const float *__restrict__ s, const int *__restrict__ tiles, const int *__restrict__ n_tiles, float *__restrict__ out)
 {
-    typedef MoeTile T;
+    typedef MoeTile<PLACES> T;
+    constexpr int MINE = 16 * T::TN;          // places of a wave
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1;
     int tile, block;
@@ -558,9 +561,9 @@ __global__ void __launch_bounds__(64 * MoeTile::WAVES, 2) k_moe_fp8_down_tile(co
     const float *sd = sdown + ((size_t)e * wb + min(nw, width - 1) / BLOCK) * fb;
     tile_sums<WIDE, 1, true, T, 2>(
         smem, ff, down + ((size_t)e * width + n0) * ff, [&](int r) { return (uint32_t)min(r, width - 1 - n0) * (uint32_t)ff; }, q + (size_t)at0 * ff,
-        [&](int r) { return (uint32_t)min(r, n_at - 1) * (uint32_t)ff; }, [&](int) { return sd; }, s + (size_t)(at0 + min(32 * wn + (lane & 31), n_at - 1)) * fb, 32 * wn >= n_at || nw >= width, acc);
+        [&](int r) { return (uint32_t)min(r, n_at - 1) * (uint32_t)ff; }, [&](int) { return sd; }, s + (size_t)(at0 + min(MINE * wn + lane % MINE, n_at - 1)) * fb, MINE * wn >= n_at || nw >= width, acc);
     tile_out<T, 4>(smem, acc, [&](int t, int n, float *v) {
-        if (32 * wn + t < n_at && nw + n < width) *reinterpret_cast<u32x4 *>(out + (size_t)(at0 + 32 * wn + t) * width + nw + n) = pack<IFA_F32>(v);          // (width in whole 16s)
+        if (MINE * wn + t < n_at && nw + n < width) *reinterpret_cast<u32x4 *>(out + (size_t)(at0 + MINE * wn + t) * width + nw + n) = pack<IFA_F32>(v);          // (width in whole 16s)
     });
 }
 
@@ -596,7 +599,7 @@ struct Work {
     int per, blocks;          // k_moe_fp8_count's
     Work(size_t rows, size_t top, size_t width, size_t ff, size_t experts)
     {
-        const size_t pairs = rows * top, n_tiles = pairs / PLACES + std::min(pairs, experts) + 1;
+        const size_t pairs = rows * top, n_tiles = pairs / 128 + std::min(pairs, experts) + 1;
         per = (int)std::max<size_t>(2048, (pairs + 255) / 256);
         blocks = (int)((pairs + per - 1) / per);
         size_t o = 0;
@@ -611,6 +614,35 @@ struct Work {
         bytes = o;
     }
 };
+
+// Places of a tile: what takes least by these figures (us, measured: a step, that is a block of 128 columns, and beside the steps), with the experts' rows scattered about their mean as independent choices
+// would be.  A tile that is not full has waves that only fetch; they leave 0.4 of a step's time to those that do not.  us 128 / 192 / 256, rows: 64 experts of 2048 x 1408, top 6, 1024 164 / 173 / 181,
+// 1400 228 / 187 / 198, 2048 255 / 242 / 216, 3001 364 / 322 / 374, 4096 453 / 417 / 398; 8 of 4096 x 4096, top 2, 700 153 / 194 / 160, 1100 228 / 186 / 212; of these and six more the choice
+// is the fastest but for one (5 %).  (32-bit outputs' products need the registers that more places would.)
+int places_for(int width, int ff, int experts, int pairs)
+{
+    constexpr struct { int places; double step, beside; } FORMS[3] = {{128, 1.05, 7.0}, {192, 1.40, 8.0}, {256, 1.78, 9.0}};
+    constexpr double SHARE[7] = {0.07, 0.12, 0.20, 0.22, 0.20, 0.12, 0.07};          // of experts (k - 3) / 2 deviations from the mean
+    const double mean = (double)pairs / experts;
+    int best = 128;
+    double least = 1e30;
+    for (const auto &F : FORMS) {
+        double us = 0.0;
+        for (int down = 0; down < 2; down++) {
+            const double steps = (double)blocks_of(down ? ff : width), blocks = down ? (width + 255) / 256 : (double)blocks_of(ff);
+            double time = 0.0, tiles = 0.0;          // an expert's
+            for (int k = 0; k < 7; k++) {
+                const double n = std::max(1.0, mean + 0.5 * (k - 3) * std::sqrt(mean)), full = std::floor(n / F.places), rest = n - full * F.places, live = std::ceil(4.0 * rest / F.places);
+                time += SHARE[k] * (full * (F.beside + steps * F.step) + (rest > 0.0 ? F.beside + steps * F.step * (0.6 + 0.1 * live) : 0.0));
+                tiles += SHARE[k] * (full + (rest > 0.0 ? 1.0 : 0.0));
+            }
+            const double rounds = experts * tiles * blocks / 256, each = time / tiles;
+            us += std::max((rounds + 0.5) * each, rounds < 3.0 ? std::ceil(rounds - 0.02) * each : 0.0);
+        }
+        if (us < least) { least = us; best = F.places; }
+    }
+    return best;
+}
 
 // what fits the kernels' 32-bit offsets, lists and grids
 bool sizes_known(size_t rows, int top, int width, int ff, int experts)
@@ -680,22 +712,23 @@ int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t ld
         IFA_LAUNCH_CHECK();
         return IFA_OK;
     }
-    // lists go through an expert's matrices once for each 32 of its rows, tiles once for each 128 but with four launches more about them.  us lists / tiles, rows: 64 experts of 2048 x 1408, top 6,
+    // lists go through an expert's matrices once for each 32 of its rows, tiles once for each 128 to 256 but with four launches more about them.  us lists / tiles, rows: 64 experts of 2048 x 1408, top 6,
     // 64 126 / 141, 100 145 / 135, 256 235 / 145; 32 of 2048 x 704, top 4, 96 47 / 50, 160 58 / 51; 16 of 1024 x 704, top 4, 64 27 / 39, 128 39 / 40, 256 60 / 41; 8 of 4096 x 4096, top 2, 48 110 / 121, 64 135 / 120
     const bool wide = y_dtype == IFA_F32, many = pairs > LIST_MAX || ff > DOWN_FF || (double)pairs / experts >= (experts * bytes > 256e6 ? 12.0 : experts * bytes > 64e6 ? 15.0 : 30.0);
     if (many) {
-        const int max_tiles = pairs / PLACES + std::min(pairs, experts);
+        const int places = wide ? 128 : places_for(width, ff, experts, pairs), max_tiles = pairs / places + std::min(pairs, experts);
+        const int lds_bytes = places == 256 ? MoeTile<256>::SMEM : places == 192 ? MoeTile<192>::SMEM : MoeTile<128>::SMEM;
         const size_t g_up = blocks_of(ff) * max_tiles, g_down = (size_t)((width + 255) / 256) * max_tiles;
-        IFA_REQUIRE(g_up < (1u << 31) && g_down < (1u << 31), "ifa_moe_experts_fp8: too many rows");
         int *counts = (int *)(base + W.counts);
         hipLaunchKernelGGL(k_moe_fp8_count, dim3(W.blocks), dim3(1024), 0, st, idx_dev, pairs, experts, W.per, counts);
-        hipLaunchKernelGGL(k_moe_fp8_place, dim3(W.blocks), dim3(1024), 0, st, idx_dev, pairs, experts, top, PLACES, W.per, counts, place_row, pair_at, tiles, n_tiles);
-        const auto fn = wide ? k_moe_fp8_down_tile<true> : k_moe_fp8_down_tile<false>;
-        IFA_HIP_CHECK(hipFuncSetAttribute((const void *)k_moe_fp8_up_tile, hipFuncAttributeMaxDynamicSharedMemorySize, MoeTile::SMEM));
-        IFA_HIP_CHECK(hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, MoeTile::SMEM));
-        hipLaunchKernelGGL(k_moe_fp8_up_tile, dim3((unsigned)g_up), dim3(64 * MoeTile::WAVES), MoeTile::SMEM, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, (const uint8_t *)a_e4m3,
-                           lda, (const float *)a_scale_f32, lds, place_row, tiles, n_tiles, glu_kind, limit, q, s);
-        hipLaunchKernelGGL(fn, dim3((unsigned)g_down), dim3(64 * MoeTile::WAVES), MoeTile::SMEM, st, (const uint8_t *)down_e4m3, (const float *)down_scale_f32, width, ff, q, s, tiles, n_tiles, out);
+        hipLaunchKernelGGL(k_moe_fp8_place, dim3(W.blocks), dim3(1024), 0, st, idx_dev, pairs, experts, top, places, W.per, counts, place_row, pair_at, tiles, n_tiles);
+        const auto up_fn = places == 256 ? k_moe_fp8_up_tile<256> : places == 192 ? k_moe_fp8_up_tile<192> : k_moe_fp8_up_tile<128>;
+        const auto fn = wide ? k_moe_fp8_down_tile<true, 128> : places == 256 ? k_moe_fp8_down_tile<false, 256> : places == 192 ? k_moe_fp8_down_tile<false, 192> : k_moe_fp8_down_tile<false, 128>;
+        IFA_HIP_CHECK(hipFuncSetAttribute((const void *)up_fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes));
+        IFA_HIP_CHECK(hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes));
+        hipLaunchKernelGGL(up_fn, dim3((unsigned)g_up), dim3(512), lds_bytes, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, (const uint8_t *)a_e4m3, lda,
+                           (const float *)a_scale_f32, lds, place_row, tiles, n_tiles, glu_kind, limit, q, s);
+        hipLaunchKernelGGL(fn, dim3((unsigned)g_down), dim3(512), lds_bytes, st, (const uint8_t *)down_e4m3, (const float *)down_scale_f32, width, ff, q, s, tiles, n_tiles, out);
     } else {
         hipLaunchKernelGGL(k_moe_fp8_up_list, dim3(ff / 16, experts), dim3(64 * LIST_WAVES), 0, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, pairs, top,
                            (const uint8_t *)a_e4m3, lda, (const float *)a_scale_f32, lds, idx_dev, glu_kind, limit, act);
