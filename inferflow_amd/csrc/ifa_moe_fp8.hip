@@ -160,6 +160,7 @@ __global__ void __launch_bounds__(64 * ROUTE_ROWS) k_moe_route_groups(const floa
 // ---- one to a few rows, two launches: every (row, choice) pair streams its expert's matrices.
 // act[p][n] = act(Gate_e a) (Up_e a) of pair p; grid (16 columns each, pairs), the blocks of columns shared out to the waves
 constexpr int PAIR_WAVES = 8;
+template <bool WIDE>
 __global__ void __launch_bounds__(64 * PAIR_WAVES) k_moe_fp8_up_pairs(const uint8_t *__restrict__ gu, const float *__restrict__ sgu, int width, int ff, int experts, int top,
                                                                       const uint8_t *__restrict__ a, size_t lda, const float *__restrict__ sa, size_t lds, const int *__restrict__ idx, int kind,
                                                                       float limit, float *__restrict__ act)
@@ -175,7 +176,7 @@ __global__ void __launch_bounds__(64 * PAIR_WAVES) k_moe_fp8_up_pairs(const uint
     const float *sar[1] = {sa + t * lds};
     f32x4 acc[2][1];
     acc[0][0] = acc[1][0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    stream_blocks<false, 1, 2, 1>(wr, swr, ar, sar, width, wave, PAIR_WAVES, acc);
+    stream_blocks<WIDE, 1, 2, 1>(wr, swr, ar, sar, width, wave, PAIR_WAVES, acc);
     join_waves<PAIR_WAVES, 2, 1>(acc, red);
     if (wave > 0 || (lane & 15)) return;          // (the sixteen activation rows of the products are one and the same)
     f32x4 v;
@@ -302,7 +303,7 @@ template <int WAVES> __device__ __forceinline__ int list_pairs(const int *__rest
 
 // act[p] of the expert's pairs; grid (16 columns each, experts), the blocks of columns shared out to the waves.  (A workgroup of 128 columns, a wave 16 of them, could quantise them too: few workgroups,
 // 22.6 + 3.4 -> 32.5 us for 53 rows of four of 32 experts, 2048 x 704.)
-template <int TILES>
+template <bool WIDE, int TILES>
 __device__ __forceinline__ void up_list(const uint16_t *list, int n, const uint8_t *const (&wr)[2], const float *const (&swr)[2], int n0, int width, int ff, int top, const uint8_t *a, size_t lda,
                                         const float *sa, size_t lds, int kind, float limit, float *act, f32x4 *red)
 {
@@ -316,7 +317,7 @@ __device__ __forceinline__ void up_list(const uint16_t *list, int n, const uint8
         ar[j] = a + t * lda; sar[j] = sa + t * lds;
         acc[0][j] = acc[1][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    stream_blocks<false, 1, 2, TILES, false>(wr, swr, ar, sar, width, wave, LIST_WAVES, acc);
+    stream_blocks<WIDE, 1, 2, TILES, false>(wr, swr, ar, sar, width, wave, LIST_WAVES, acc);
     join_waves<LIST_WAVES, 2, TILES>(acc, red);
     if (wave == 0) {
 #pragma unroll
@@ -330,6 +331,7 @@ __device__ __forceinline__ void up_list(const uint16_t *list, int n, const uint8
     }
     __syncthreads();          // (`red` is read)
 }
+template <bool WIDE>
 __global__ void __launch_bounds__(64 * LIST_WAVES) k_moe_fp8_up_list(const uint8_t *__restrict__ gu, const float *__restrict__ sgu, int width, int ff, int pairs, int top,
                                                                      const uint8_t *__restrict__ a, size_t lda, const float *__restrict__ sa, size_t lds, const int *__restrict__ idx, int kind,
                                                                      float limit, float *__restrict__ act)
@@ -342,8 +344,8 @@ __global__ void __launch_bounds__(64 * LIST_WAVES) k_moe_fp8_up_list(const uint8
     const uint8_t *wr[2] = {gu + ((size_t)e * 2 * ff + r0) * width, gu + ((size_t)(e * 2 + 1) * ff + r0) * width};
     const float *swr[2] = {sgu + ((size_t)e * 2 * fb + n0 / BLOCK) * wb, sgu + ((size_t)(e * 2 + 1) * fb + n0 / BLOCK) * wb};
     for (int at = 0; at < n; at += 32) {
-        if (n - at <= 16) up_list<1>(list + at, n - at, wr, swr, n0, width, ff, top, a, lda, sa, lds, kind, limit, act, red);
-        else up_list<2>(list + at, n - at, wr, swr, n0, width, ff, top, a, lda, sa, lds, kind, limit, act, red);
+        if (n - at <= 16) up_list<WIDE, 1>(list + at, n - at, wr, swr, n0, width, ff, top, a, lda, sa, lds, kind, limit, act, red);
+        else up_list<WIDE, 2>(list + at, n - at, wr, swr, n0, width, ff, top, a, lda, sa, lds, kind, limit, act, red);
     }
 }
 
@@ -477,7 +479,7 @@ __device__ __forceinline__ bool moe_tile(const int *n_tiles, int blocks, int &ti
 }
 
 // a tile of 128 gate rows and the 128 up rows of the same columns: one block of the activations, which leave it quantised
-template <int PLACES>
+template <bool WIDE, int PLACES>
 __global__ void __launch_bounds__(512, 2) k_moe_fp8_up_tile(const uint8_t *__restrict__ gu, const float *__restrict__ sgu, int width, int ff, const uint8_t *__restrict__ a, size_t lda,
                                                             const float *__restrict__ sa, size_t lds, const int *__restrict__ place_row, const int *__restrict__ tiles,
                                                             const int *__restrict__ n_tiles, int kind, float limit, uint8_t *__restrict__ q, float *__restrict__ s)
@@ -497,7 +499,7 @@ __global__ void __launch_bounds__(512, 2) k_moe_fp8_up_tile(const uint8_t *__res
     const size_t wb = blocks_of(width);
     const float *sg = sgu + ((size_t)e * 2 * fb + block) * wb, *su = sg + fb * wb;
     auto row_of = [&](int r) { return (size_t)place_row[at0 + min(r, n_at - 1)]; };
-    tile_sums<false, 2, false, T, 2>(
+    tile_sums<WIDE, 2, false, T, 2>(
         smem, width, gu + (size_t)e * 2 * ff * width, [&](int r) { return (uint32_t)((r < BLOCK ? 0 : ff) + min(n0 + (r & (BLOCK - 1)), ff - 1)) * (uint32_t)width; }, nullptr,
         [&](int r) { return a + row_of(r) * lda; }, [&](int h) { return h ? su : sg; }, sa + row_of(MINE * wn + lane % MINE) * lds, MINE * wn >= n_at, acc);
     lds_barrier();          // (the buffers' last block is read)
@@ -618,22 +620,24 @@ struct Work {
 // Places of a tile: what takes least by these figures (us, measured: a step, that is a block of 128 columns, and beside the steps), with the experts' rows scattered about their mean as independent choices
 // would be.  A tile that is not full has waves that only fetch; they leave 0.4 of a step's time to those that do not.  us 128 / 192 / 256, rows: 64 experts of 2048 x 1408, top 6, 1024 164 / 173 / 181,
 // 1400 228 / 187 / 198, 2048 255 / 242 / 216, 3001 364 / 322 / 374, 4096 453 / 417 / 398; 8 of 4096 x 4096, top 2, 700 153 / 194 / 160, 1100 228 / 186 / 212; of these and six more the choice
-// is the fastest but for one (5 %).  (32-bit outputs' products need the registers that more places would.)
-int places_for(int width, int ff, int experts, int pairs)
+// is the fastest but for one (5 %).  exact: gate and up, wide: down on exact halves (256 places do not fit the registers then); 128 / 192, halves, 1400 rows 288 / 234, 2048 336 / 359, 3001 483 / 453, 32-bit
+// 316 / 245, 371 / 403, 532 / 477; of these and twelve more the choice is 0.9 % behind on average.
+int places_for(int width, int ff, int experts, int pairs, bool exact, bool wide)
 {
-    constexpr struct { int places; double step, beside; } FORMS[3] = {{128, 1.05, 7.0}, {192, 1.40, 8.0}, {256, 1.78, 9.0}};
+    constexpr struct { int places; double step, exact, beside; } FORMS[3] = {{128, 1.05, 1.7, 7.0}, {192, 1.40, 2.0, 8.0}, {256, 1.78, 0.0, 9.0}};
     constexpr double SHARE[7] = {0.07, 0.12, 0.20, 0.22, 0.20, 0.12, 0.07};          // of experts (k - 3) / 2 deviations from the mean
     const double mean = (double)pairs / experts;
     int best = 128;
     double least = 1e30;
     for (const auto &F : FORMS) {
+        if (exact && F.exact == 0.0) continue;
         double us = 0.0;
         for (int down = 0; down < 2; down++) {
-            const double steps = (double)blocks_of(down ? ff : width), blocks = down ? (width + 255) / 256 : (double)blocks_of(ff);
+            const double steps = (double)blocks_of(down ? ff : width), blocks = down ? (width + 255) / 256 : (double)blocks_of(ff), step = (down ? wide : exact) ? F.exact : F.step;
             double time = 0.0, tiles = 0.0;          // an expert's
             for (int k = 0; k < 7; k++) {
                 const double n = std::max(1.0, mean + 0.5 * (k - 3) * std::sqrt(mean)), full = std::floor(n / F.places), rest = n - full * F.places, live = std::ceil(4.0 * rest / F.places);
-                time += SHARE[k] * (full * (F.beside + steps * F.step) + (rest > 0.0 ? F.beside + steps * F.step * (0.6 + 0.1 * live) : 0.0));
+                time += SHARE[k] * (full * (F.beside + steps * step) + (rest > 0.0 ? F.beside + steps * step * (0.6 + 0.1 * live) : 0.0));
                 tiles += SHARE[k] * (full + (rest > 0.0 ? 1.0 : 0.0));
             }
             const double rounds = experts * tiles * blocks / 256, each = time / tiles;
@@ -702,8 +706,11 @@ int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t ld
     // one or two rows, or up to four of small matrices: a stream for each pair.  us pairs / lists, rows x choices of experts, width x ff: 1 x 6 of 64, 2048 x 1408 20.6 / 33.5, 2 28.1 / 37.6, 4 48.4 / 47.8;
     // 4 x 4 of 16, 1024 x 704 14.9 / 17.2, 8 25.5 / 18.4; 2 x 2 of 8, 4096 x 4096 54 / 55, 3 76 / 64
     const double bytes = 3.0 * width * ff;
+    // Gate and up decide which e4m3 value an activation becomes: the 8-bit instructions' error moves one in some thousands to its neighbour, 1e-3 of the output.  That is below a bfloat16's rounding; for a half's
+    // or a 32-bit output both run on exact halves, gate and up for the former, down too for the latter (ifa_fp8.h).
+    const bool exact = y_dtype != IFA_BF16, wide = y_dtype == IFA_F32;
     if ((rows <= 2 || (rows <= 4 && bytes <= 4e6)) && few_lds <= 48 * 1024) {
-        hipLaunchKernelGGL(k_moe_fp8_up_pairs, dim3(ff / 16, pairs), dim3(64 * PAIR_WAVES), 0, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, experts, top,
+        hipLaunchKernelGGL(exact ? k_moe_fp8_up_pairs<true> : k_moe_fp8_up_pairs<false>, dim3(ff / 16, pairs), dim3(64 * PAIR_WAVES), 0, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, experts, top,
                            (const uint8_t *)a_e4m3, lda, (const float *)a_scale_f32, lds, idx_dev, glu_kind, limit, act);
 #define IFA_DOWN(DT) hipLaunchKernelGGL((k_moe_fp8_down_pairs<DT, 3>), dim3(width / 8, (unsigned)rows), dim3(64 * PAIR_WAVES), few_lds, st, (const uint8_t *)down_e4m3, (const float *)down_scale_f32, \
                                         width, ff, experts, top, act, idx_dev, (const float *)wgt_f32, (Elem<DT>::type *)y, ldy, accumulate)
@@ -714,23 +721,23 @@ int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t ld
     }
     // lists go through an expert's matrices once for each 32 of its rows, tiles once for each 128 to 256 but with four launches more about them.  us lists / tiles, rows: 64 experts of 2048 x 1408, top 6,
     // 64 126 / 141, 100 145 / 135, 256 235 / 145; 32 of 2048 x 704, top 4, 96 47 / 50, 160 58 / 51; 16 of 1024 x 704, top 4, 64 27 / 39, 128 39 / 40, 256 60 / 41; 8 of 4096 x 4096, top 2, 48 110 / 121, 64 135 / 120
-    const bool wide = y_dtype == IFA_F32, many = pairs > LIST_MAX || ff > DOWN_FF || (double)pairs / experts >= (experts * bytes > 256e6 ? 12.0 : experts * bytes > 64e6 ? 15.0 : 30.0);
+    const bool many = pairs > LIST_MAX || ff > DOWN_FF || (double)pairs / experts >= (experts * bytes > 256e6 ? 12.0 : experts * bytes > 64e6 ? 15.0 : 30.0);
     if (many) {
-        const int places = wide ? 128 : places_for(width, ff, experts, pairs), max_tiles = pairs / places + std::min(pairs, experts);
+        const int places = places_for(width, ff, experts, pairs, exact, wide), max_tiles = pairs / places + std::min(pairs, experts);
         const int lds_bytes = places == 256 ? MoeTile<256>::SMEM : places == 192 ? MoeTile<192>::SMEM : MoeTile<128>::SMEM;
         const size_t g_up = blocks_of(ff) * max_tiles, g_down = (size_t)((width + 255) / 256) * max_tiles;
         int *counts = (int *)(base + W.counts);
         hipLaunchKernelGGL(k_moe_fp8_count, dim3(W.blocks), dim3(1024), 0, st, idx_dev, pairs, experts, W.per, counts);
         hipLaunchKernelGGL(k_moe_fp8_place, dim3(W.blocks), dim3(1024), 0, st, idx_dev, pairs, experts, top, places, W.per, counts, place_row, pair_at, tiles, n_tiles);
-        const auto up_fn = places == 256 ? k_moe_fp8_up_tile<256> : places == 192 ? k_moe_fp8_up_tile<192> : k_moe_fp8_up_tile<128>;
-        const auto fn = wide ? k_moe_fp8_down_tile<true, 128> : places == 256 ? k_moe_fp8_down_tile<false, 256> : places == 192 ? k_moe_fp8_down_tile<false, 192> : k_moe_fp8_down_tile<false, 128>;
+        const auto up_fn = exact ? (places == 192 ? k_moe_fp8_up_tile<true, 192> : k_moe_fp8_up_tile<true, 128>) : places == 256 ? k_moe_fp8_up_tile<false, 256> : places == 192 ? k_moe_fp8_up_tile<false, 192> : k_moe_fp8_up_tile<false, 128>;
+        const auto fn = wide ? (places == 192 ? k_moe_fp8_down_tile<true, 192> : k_moe_fp8_down_tile<true, 128>) : places == 256 ? k_moe_fp8_down_tile<false, 256> : places == 192 ? k_moe_fp8_down_tile<false, 192> : k_moe_fp8_down_tile<false, 128>;
         IFA_HIP_CHECK(hipFuncSetAttribute((const void *)up_fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes));
         IFA_HIP_CHECK(hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes));
         hipLaunchKernelGGL(up_fn, dim3((unsigned)g_up), dim3(512), lds_bytes, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, (const uint8_t *)a_e4m3, lda,
                            (const float *)a_scale_f32, lds, place_row, tiles, n_tiles, glu_kind, limit, q, s);
         hipLaunchKernelGGL(fn, dim3((unsigned)g_down), dim3(512), lds_bytes, st, (const uint8_t *)down_e4m3, (const float *)down_scale_f32, width, ff, q, s, tiles, n_tiles, out);
     } else {
-        hipLaunchKernelGGL(k_moe_fp8_up_list, dim3(ff / 16, experts), dim3(64 * LIST_WAVES), 0, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, pairs, top,
+        hipLaunchKernelGGL(exact ? k_moe_fp8_up_list<true> : k_moe_fp8_up_list<false>, dim3(ff / 16, experts), dim3(64 * LIST_WAVES), 0, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, pairs, top,
                            (const uint8_t *)a_e4m3, lda, (const float *)a_scale_f32, lds, idx_dev, glu_kind, limit, act);
         const auto fn = wide ? k_moe_fp8_down_list<true> : k_moe_fp8_down_list<false>;
         const size_t list_lds = 16 * blocks_of(ff) * (BLOCK + 4);
