@@ -1,5 +1,6 @@
 // ifa_fp8_stream.h -- products of a few rows in 8-bit floating point: sixteen matrix rows against TILES x 16 activation rows, the blocks of 128 columns one after the other or shared out
 // to waves.  Bound by the matrix's bytes: they go from memory to registers, DEPTH blocks asked for while DEPTH blocks are multiplied.
+// One row, 4096 x 11008 from memory: 10.6 us, 4.3 TB/s with the launch's start and end (a large copy: 4.9); two blocks asked for at a time or 32 matrix rows a workgroup: no faster.
 #pragma once
 #include "ifa_fp8.h"
 

@@ -7,6 +7,8 @@
 //     other matrix rows at its end.  So every request has one and a half blocks' products to arrive under (one block's: 2.1 us a block of a 256 x 256 tile instead of 1.8; two and a half, a third buffer
 //     of 256 x 128 tiles: 1.13 instead of 1.11);
 //   * the requests are inline assembly without results (the compiler would wait for all of them in front of every read of LDS); the waits and barriers stand beside them.
+// Measured: 256 x 256 tiles, 4096 rows of 4096 x 16384 2.25-2.32 PFLOP/s, where the chip's power limit lowers its clock (a lone workgroup 1.46 us a block, 0.85 of them products); 11008 x 4096 1.9
+// (688 tiles on 256 compute units).
 // Columns beyond the last block's end: the requests stay inside their row, and zeros are written over what they brought.  Rows beyond the last: repeated, not stored.
 #pragma once
 #include "ifa_fp8.h"
