@@ -80,7 +80,7 @@ __device__ __forceinline__ uint32_t quantise4(const float *v, float inv)
 // ---- gated activations f(a, u): kind 0 a sigmoid(a) u, 1 gelu's tanh form (= a sigmoid(2 sqrt(2 / pi) (a + 0.044715 a^3))) u, 2 max(a, 0) u, 3 a' sigmoid(1.702 a') (u' + 1) with a' = min(a, limit),
 // u' = u within +- limit; a NaN stays one.  sigmoid(x) = 1 / (1 + 2^t), t = -x log2(e): its rounding put right through the exponential's derivative, one instruction for the power of two and one
 // for the reciprocal (1 unit in the last place each).  t goes no further than the largest power, where the reciprocal is 0.  (With the library's exponential and a correctly rounded
-// quotient, 40 instructions a value instead of 17, the row kernel waits for instructions and not for memory: 2051 x 11008 bf16 28.0 us, so 22.9.)
+// quotient, 40 instructions a value instead of 17, the row kernel waits for instructions and not for memory: 2051 x 11008 bf16 28.0 us, so 22.3.)
 __device__ __forceinline__ float sigmoid(float x)
 {
     constexpr float L = 1.44269504f, L_REST = 1.92596303e-08f, LN2 = 0.69314718f;      // log2(e) = L + L_REST
@@ -88,13 +88,22 @@ __device__ __forceinline__ float sigmoid(float x)
     const float e = __builtin_amdgcn_exp2f(t);
     return __builtin_amdgcn_rcpf(1.0f + fmaf(e, LN2 * fmaf(y, L_REST, fmaf(y, L, -t)), e));
 }
-__device__ __forceinline__ float gated(int kind, float limit, float a, float u)
+template <int KIND> __device__ __forceinline__ float gated(float limit, float a, float u)
 {
-    if (kind == 0) return a * sigmoid(a) * u;
-    if (kind == 1) return a * sigmoid(a * fmaf(a * a, 0.0713548163f, 1.59576912f)) * u;
-    if (kind == 2) return (a < 0.0f ? 0.0f : a) * u;
-    const float ac = a > limit ? limit : a, uc = u > limit ? limit : u < -limit ? -limit : u;
-    return ac * sigmoid(1.702f * ac) * (uc + 1.0f);
+    if constexpr (KIND == 0) return a * sigmoid(a) * u;
+    else if constexpr (KIND == 1) return a * sigmoid(a * fmaf(a * a, 0.0713548163f, 1.59576912f)) * u;
+    else if constexpr (KIND == 2) return (a < 0.0f ? 0.0f : a) * u;
+    else {
+        const float ac = a > limit ? limit : a, uc = u > limit ? limit : u < -limit ? -limit : u;
+        return ac * sigmoid(1.702f * ac) * (uc + 1.0f);
+    }
+}
+// a[i] = f(a[i], u[i]): one look at the kind for all of them, so that their exponentials run beside each other
+template <int N> __device__ __forceinline__ void gated_all(int kind, float limit, float (&a)[N], const float (&u)[N])
+{
+#define IFA_GATED(K) { _Pragma("unroll") for (int i = 0; i < N; i++) a[i] = gated<K>(limit, a[i], u[i]); }
+    if (kind == 0) IFA_GATED(0) else if (kind == 1) IFA_GATED(1) else if (kind == 2) IFA_GATED(2) else IFA_GATED(3)
+#undef IFA_GATED
 }
 // maximum over aligned groups of LANES lanes (16 or 32); every lane gets it
 __device__ __forceinline__ uint32_t dpp_max(uint32_t v, uint32_t o) { return v > o ? v : o; }

@@ -64,8 +64,8 @@ __global__ void __launch_bounds__(1024) k_norm_add_fp8(typename Elem<DT>::type *
 }
 
 // a thread a piece; pieces of a row padded to whole blocks so that a block's lanes stay together
-template <int DT>
-__global__ void __launch_bounds__(256) k_glu_fp8(int kind, float limit, const typename Elem<DT>::type *__restrict__ gu, size_t ld, int cols, int pieces, size_t all,
+template <int DT, int KIND>
+__global__ void __launch_bounds__(256) k_glu_fp8(float limit, const typename Elem<DT>::type *__restrict__ gu, size_t ld, int cols, int pieces, size_t all,
                                                  uint8_t *__restrict__ q, size_t ldq, float *__restrict__ scale, size_t lds)
 {
     constexpr int N = VEC<DT>;
@@ -77,11 +77,11 @@ __global__ void __launch_bounds__(256) k_glu_fp8(int kind, float limit, const ty
     uint32_t most = 0u;
     if (live) {
         unpack<DT>(*reinterpret_cast<const u32x4 *>(gu + t * ld + c), v);
-        if (kind != 4) {
+        if constexpr (KIND != 4) {
             float u[N];
             unpack<DT>(*reinterpret_cast<const u32x4 *>(gu + t * ld + cols + c), u);
 #pragma unroll
-            for (int e = 0; e < N; e++) v[e] = gated(kind, limit, v[e], u[e]);
+            for (int e = 0; e < N; e++) v[e] = gated<KIND>(limit, v[e], u[e]);
         }
 #pragma unroll
         for (int e = 0; e < N; e++) most = dpp_max(most, abs_bits(v[e]));
@@ -121,7 +121,8 @@ int glu(int kind, float limit, const void *gu, size_t ld, size_t rows, size_t co
 {
     typedef typename Elem<DT>::type T;
     const size_t pieces = blocks_of(cols) * (BLOCK / VEC<DT>), all = rows * pieces;
-    hipLaunchKernelGGL((k_glu_fp8<DT>), dim3((unsigned)((all + 255) / 256)), dim3(256), 0, s, kind, limit, (const T *)gu, ld, (int)cols, (int)pieces, all, (uint8_t *)q, ldq,
+    const auto fn = kind == 0 ? k_glu_fp8<DT, 0> : kind == 1 ? k_glu_fp8<DT, 1> : kind == 2 ? k_glu_fp8<DT, 2> : kind == 3 ? k_glu_fp8<DT, 3> : k_glu_fp8<DT, 4>;
+    hipLaunchKernelGGL(fn, dim3((unsigned)((all + 255) / 256)), dim3(256), 0, s, limit, (const T *)gu, ld, (int)cols, (int)pieces, all, (uint8_t *)q, ldq,
                        (float *)scale, lds);
     IFA_LAUNCH_CHECK();
     return IFA_OK;

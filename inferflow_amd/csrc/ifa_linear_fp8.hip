@@ -57,6 +57,17 @@ __global__ void __launch_bounds__(64 * WAVES) k_linear_fp8_stream(const uint8_t 
     }
 }
 
+struct LinearJob {
+    const uint8_t *wbase, *abase;
+    const float *swr, *sa;
+    int cols, row_cols, last_row, last_token, nw, tw, part;          // (nw, tw: the wave's first rows)
+    uint32_t lda;
+    bool idle;
+    __device__ __forceinline__ uint32_t woff(int r) const { return (uint32_t)min(r, last_row) * (uint32_t)row_cols; }
+    __device__ __forceinline__ uint32_t asrc(int r) const { return (uint32_t)min(r, last_token) * lda; }
+    __device__ __forceinline__ const float *sw(int) const { return swr; }
+};
+
 template <int DT, class T, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, 2) k_linear_fp8_tile(const uint8_t *__restrict__ w, const float *__restrict__ sw, int rows, int cols, const uint8_t *__restrict__ a, size_t lda,
                                                                      const float *__restrict__ sa, size_t lds, int tokens, const bf16_t *__restrict__ bias, int accumulate,
@@ -67,51 +78,55 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_linear_fp8_tile(const uint8
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % WM, wn = wave / WM;
     // bands of eight activation tiles, the tiles of a band fastest; the parts of the columns one behind the other
-    const int tiles = tiles_t * tiles_n, part = blockIdx.x / tiles, at = xcd_place(blockIdx.x - part * tiles, tiles), band = at / (BAND * tiles_n), within = at % (BAND * tiles_n);
-    const int band_t = min(BAND, tiles_t - band * BAND), t0 = (band * BAND + within % band_t) * BN, n0 = within / band_t * BM;
-    const int nb = (cols + BLOCK - 1) / BLOCK, b0 = (int)((long long)part * nb / parts), b1 = (int)((long long)(part + 1) * nb / parts);
-    f32x4 acc[T::TM][T::TN];
-#pragma unroll
-    for (int j = 0; j < T::TN; j++)
-#pragma unroll
-        for (int m = 0; m < T::TM; m++) acc[m][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const int nw = n0 + wm * (BM / WM), tw = t0 + wn * (BN / WN);          // the wave's first rows
-    const float *swr = sw + (size_t)(min(nw, rows - 1) / BLOCK) * blocks_of(cols);
-    tile_sums<DT == IFA_F32, 1, true, T, WM>(
-        smem, min(cols, b1 * BLOCK) - b0 * BLOCK, w + (size_t)n0 * cols + (size_t)b0 * BLOCK, [&](int r) { return (uint32_t)min(r, rows - 1 - n0) * (uint32_t)cols; },
-        a + (size_t)t0 * lda + (size_t)b0 * BLOCK, [&](int r) { return (uint32_t)min(r, tokens - 1 - t0) * (uint32_t)lda; }, [&](int) { return swr + b0; },
-        sa + (size_t)min(tw + lane % (16 * T::TN), tokens - 1) * lds + b0, tw >= tokens || nw >= rows, acc);
-    if (parts > 1) {
-        float *const plane = planes + (size_t)part * tokens * rows;
-        tile_out<T, 4>(smem, acc, [&](int t, int n, float *v) {
+    const int tiles = tiles_t * tiles_n, nb = (cols + BLOCK - 1) / BLOCK;
+    const Share share(tiles * parts);
+    auto job = [&](int k) {
+        LinearJob J;
+        const int place = share.at(k), part = place / tiles, at = place - part * tiles, band = at / (BAND * tiles_n), within = at % (BAND * tiles_n), band_t = min(BAND, tiles_t - band * BAND);
+        const int t0 = (band * BAND + within % band_t) * BN, n0 = within / band_t * BM;
+        const int b0 = (int)((long long)part * nb / parts), b1 = (int)((long long)(part + 1) * nb / parts);
+        J.part = part; J.nw = n0 + wm * (BM / WM); J.tw = t0 + wn * (BN / WN);
+        J.cols = min(cols, b1 * BLOCK) - b0 * BLOCK; J.row_cols = cols; J.last_row = rows - 1 - n0; J.last_token = tokens - 1 - t0; J.lda = (uint32_t)lda;
+        J.wbase = w + (size_t)n0 * cols + (size_t)b0 * BLOCK; J.abase = a + (size_t)t0 * lda + (size_t)b0 * BLOCK;
+        J.swr = sw + (size_t)(min(J.nw, rows - 1) / BLOCK) * blocks_of(cols) + b0;
+        J.sa = sa + (size_t)min(J.tw + lane % (16 * T::TN), tokens - 1) * lds + b0;
+        J.idle = J.tw >= tokens || J.nw >= rows;
+        return J;
+    };
+    tile_run<false, DT == IFA_F32, 1, true, T, WM>(smem, 1, job, [&](const LinearJob &J, const f32x4 (&acc)[T::TM][T::TN], char *buffer) {
+        const int tw = J.tw, nw = J.nw, part = J.part;
+        if (parts > 1) {
+            float *const plane = planes + (size_t)part * tokens * rows;
+            tile_out<T, false, 4>(buffer, acc, [&](int t, int n, float *v) {
+                t += tw; n += nw;
+                if (t >= tokens || n >= rows) return;
+                float *d = plane + (size_t)t * rows + n;
+                if (rows % 4 == 0) *reinterpret_cast<u32x4 *>(d) = pack<IFA_F32>(v);
+                else for (int e = 0; e < 4; e++) if (n + e < rows) d[e] = v[e];
+            });
+            return;
+        }
+        constexpr int N = VEC<DT>;
+        if (whole) tile_out<T, false, N>(buffer, acc, [&](int t, int n, float *v) {
             t += tw; n += nw;
             if (t >= tokens || n >= rows) return;
-            float *d = plane + (size_t)t * rows + n;
-            if (rows % 4 == 0) *reinterpret_cast<u32x4 *>(d) = pack<IFA_F32>(v);
-            else for (int e = 0; e < 4; e++) if (n + e < rows) d[e] = v[e];
+            typename Elem<DT>::type *d = c + (size_t)t * ldc + n;
+            if (bias) {
+#pragma unroll
+                for (int e = 0; e < N; e++) v[e] += ifa32::bf2f(bias[n + e]);
+            }
+            if (accumulate) {
+                float old[N];
+                unpack<DT>(*reinterpret_cast<const u32x4 *>(d), old);
+#pragma unroll
+                for (int e = 0; e < N; e++) v[e] += old[e];
+            }
+            *reinterpret_cast<u32x4 *>(d) = pack<DT>(v);
         });
-        return;
-    }
-    constexpr int N = VEC<DT>;
-    if (whole) tile_out<T, N>(smem, acc, [&](int t, int n, float *v) {
-        t += tw; n += nw;
-        if (t >= tokens || n >= rows) return;
-        typename Elem<DT>::type *d = c + (size_t)t * ldc + n;
-        if (bias) {
-#pragma unroll
-            for (int e = 0; e < N; e++) v[e] += ifa32::bf2f(bias[n + e]);
-        }
-        if (accumulate) {
-            float old[N];
-            unpack<DT>(*reinterpret_cast<const u32x4 *>(d), old);
-#pragma unroll
-            for (int e = 0; e < N; e++) v[e] += old[e];
-        }
-        *reinterpret_cast<u32x4 *>(d) = pack<DT>(v);
-    });
-    else tile_out<T, 1>(smem, acc, [&](int t, int n, float *v) {          // (rows that do not start on 16 bytes: a lane a value, so that a store is of neighbours all the same)
-        t += tw; n += nw;
-        if (t < tokens && n < rows) store_out<DT>(c + (size_t)t * ldc + n, v[0] + (bias ? ifa32::bf2f(bias[n]) : 0.0f), accumulate);
+        else tile_out<T, false, 1>(buffer, acc, [&](int t, int n, float *v) {          // (rows that do not start on 16 bytes: a lane a value, so that a store is of neighbours all the same)
+            t += tw; n += nw;
+            if (t < tokens && n < rows) store_out<DT>(c + (size_t)t * ldc + n, v[0] + (bias ? ifa32::bf2f(bias[n]) : 0.0f), accumulate);
+        });
     });
 }
 

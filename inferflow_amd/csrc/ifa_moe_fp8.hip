@@ -180,10 +180,9 @@ __global__ void __launch_bounds__(64 * PAIR_WAVES) k_moe_fp8_up_pairs(const uint
     stream_blocks<WIDE, 1, 2, 1>(wr, swr, ar, sar, width, wave, PAIR_WAVES, acc);
     join_waves<PAIR_WAVES, 2, 1>(acc, red);
     if (wave > 0 || (lane & 15)) return;          // (the sixteen activation rows of the products are one and the same)
-    f32x4 v;
-#pragma unroll
-    for (int r = 0; r < 4; r++) v[r] = gated(kind, limit, acc[0][0][r], acc[1][0][r]);
-    *reinterpret_cast<f32x4 *>(act + (size_t)p * ff + n0 + 4 * (lane >> 4)) = v;
+    float v[4] = {acc[0][0][0], acc[0][0][1], acc[0][0][2], acc[0][0][3]};
+    gated_all(kind, limit, v, {acc[1][0][0], acc[1][0][1], acc[1][0][2], acc[1][0][3]});
+    *reinterpret_cast<u32x4 *>(act + (size_t)p * ff + n0 + 4 * (lane >> 4)) = pack<IFA_F32>(v);
 }
 
 // 32-bit activations of pairs into e4m3 in LDS: item it = block it % fb of pair pair(it / fb) (-1: zeros); [items] blocks of 128 bytes and their scales.  Half a wave an item.
@@ -325,10 +324,9 @@ __device__ __forceinline__ void up_list(const uint16_t *list, int n, const uint8
 #pragma unroll
         for (int j = 0; j < TILES; j++) {
             if (16 * j + i >= n) continue;
-            f32x4 v;
-#pragma unroll
-            for (int r = 0; r < 4; r++) v[r] = gated(kind, limit, acc[0][j][r], acc[1][j][r]);
-            *reinterpret_cast<f32x4 *>(act + (size_t)list[16 * j + i] * ff + n0 + 4 * (lane >> 4)) = v;
+            float v[4] = {acc[0][j][0], acc[0][j][1], acc[0][j][2], acc[0][j][3]};
+            gated_all(kind, limit, v, {acc[1][j][0], acc[1][j][1], acc[1][j][2], acc[1][j][3]});
+            *reinterpret_cast<u32x4 *>(act + (size_t)list[16 * j + i] * ff + n0 + 4 * (lane >> 4)) = pack<IFA_F32>(v);
         }
     }
     __syncthreads();          // (`red` is read)
@@ -465,23 +463,41 @@ __global__ void __launch_bounds__(1024) k_moe_fp8_place(const int *__restrict__ 
     }
 }
 
-// Tiles of 128, 192 or 256 places of one expert (places_for).  A workgroup of eight waves, one a compute unit.
+// Tiles of 128 or 192 places of one expert (places_for).  A workgroup of eight waves, one a compute unit.
 template <int PLACES> using MoeTile = Tile<256, PLACES, 2, 4>;
 
-// the tile's place among those that there are (the empty ones behind them are dealt to nobody); tiles of one expert side by side
-__device__ __forceinline__ bool moe_tile(const int *n_tiles, int blocks, int &tile, int &block)
+// tile and block of columns at a place among those that there are (the empty tiles behind them are dealt to nobody): tiles of one expert side by side, full and other ones in turn for a workgroup
+__device__ __forceinline__ void moe_place(int at, int n_tiles, int blocks, int &tile, int &block)
 {
-    const int nt = *n_tiles, all = nt * blocks;
-    if ((int)blockIdx.x >= all) return false;
     constexpr int BAND = 8;
-    const int at = xcd_place(blockIdx.x, all), band = at / (BAND * blocks), within = at % (BAND * blocks), in_band = min(BAND, nt - band * BAND);
-    tile = band * BAND + within % in_band;
+    const int band = at / (BAND * blocks), within = at % (BAND * blocks), in_band = min(BAND, n_tiles - band * BAND);
     block = within / in_band;
-    return true;
+    tile = band * BAND + (within + block / 4) % in_band;
 }
 
+struct UpJob {
+    const uint8_t *wbase, *abase, *a;
+    const float *sg, *su, *sa;
+    const int *rows;          // of the tile's places
+    int cols, n0, ff, at0, n_at, block;
+    size_t lda;
+    bool idle;
+    __device__ __forceinline__ uint32_t woff(int r) const { return (uint32_t)((r < BLOCK ? 0 : ff) + min(n0 + (r & (BLOCK - 1)), ff - 1)) * (uint32_t)cols; }
+    __device__ __forceinline__ const uint8_t *asrc(int r) const { return a + (size_t)rows[min(r, n_at - 1)] * lda; }
+    __device__ __forceinline__ const float *sw(int h) const { return h ? su : sg; }
+};
+struct DownJob {
+    const uint8_t *wbase, *abase;
+    const float *sd, *sa;
+    int cols, last_row, at0, n_at, nw;          // (nw: the wave's first column)
+    bool idle;
+    __device__ __forceinline__ uint32_t woff(int r) const { return (uint32_t)min(r, last_row) * (uint32_t)cols; }
+    __device__ __forceinline__ uint32_t asrc(int r) const { return (uint32_t)min(r, n_at - 1) * (uint32_t)cols; }
+    __device__ __forceinline__ const float *sw(int) const { return sd; }
+};
+
 // a tile of 128 gate rows and the 128 up rows of the same columns: one block of the activations, which leave it quantised.  Bound by the products and a tile's ends (16 blocks of columns
-// between them): 17100 pairs of 64 experts, 2048 x 1408, 209 us
+// between them): 17100 pairs of 64 experts, 2048 x 1408, 181 us
 template <bool WIDE, int PLACES>
 __global__ void __launch_bounds__(512, 2) k_moe_fp8_up_tile(const uint8_t *__restrict__ gu, const float *__restrict__ sgu, int width, int ff, const uint8_t *__restrict__ a, size_t lda,
                                                             const float *__restrict__ sa, size_t lds, const int *__restrict__ place_row, const int *__restrict__ tiles,
@@ -491,58 +507,64 @@ __global__ void __launch_bounds__(512, 2) k_moe_fp8_up_tile(const uint8_t *__res
     constexpr int MINE = 16 * T::TN;          // places of a wave
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1, g = lane >> 4, i = lane & 15, fb = (int)blocks_of(ff);
-    int tile, block;
-    if (!moe_tile(n_tiles, fb, tile, block)) return;
-    const int e = tiles[3 * tile], at0 = tiles[3 * tile + 1], n_at = tiles[3 * tile + 2], n0 = block * BLOCK;
-    f32x4 acc[T::TM][T::TN];
-#pragma unroll
-    for (int m = 0; m < T::TM; m++)
-#pragma unroll
-        for (int j = 0; j < T::TN; j++) acc[m][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int n = *n_tiles;
+    const Share share(n * fb);
+    if (share.count == 0) return;
     const size_t wb = blocks_of(width);
-    const float *sg = sgu + ((size_t)e * 2 * fb + block) * wb, *su = sg + fb * wb;
-    auto row_of = [&](int r) { return (size_t)place_row[at0 + min(r, n_at - 1)]; };
-    tile_sums<WIDE, 2, false, T, 2>(
-        smem, width, gu + (size_t)e * 2 * ff * width, [&](int r) { return (uint32_t)((r < BLOCK ? 0 : ff) + min(n0 + (r & (BLOCK - 1)), ff - 1)) * (uint32_t)width; }, nullptr,
-        [&](int r) { return a + row_of(r) * lda; }, [&](int h) { return h ? su : sg; }, sa + row_of(MINE * wn + lane % MINE) * lds, MINE * wn >= n_at, acc);
-    lds_barrier();          // (the buffers' last block is read)
-    uint32_t *const most = reinterpret_cast<uint32_t *>(smem + PLACES * BLOCK);          // [2 waves][PLACES], behind the tile's quantised rows
-    const bool whole = n0 + BLOCK <= ff;
-    uint32_t mine[T::TN];
+    auto job = [&](int k) {
+        UpJob J;
+        int tile;
+        moe_place(share.at(k), n, fb, tile, J.block);
+        const int e = tiles[3 * tile];
+        J.at0 = tiles[3 * tile + 1]; J.n_at = tiles[3 * tile + 2]; J.n0 = J.block * BLOCK; J.cols = width; J.ff = ff; J.a = a; J.lda = lda; J.abase = nullptr;
+        J.rows = place_row + J.at0;
+        J.wbase = gu + (size_t)e * 2 * ff * width;
+        J.sg = sgu + ((size_t)e * 2 * fb + J.block) * wb; J.su = J.sg + fb * wb;
+        J.sa = sa + (size_t)J.rows[min(MINE * wn + (fresh(lane) & 63) % MINE, J.n_at - 1)] * lds;
+        J.idle = MINE * wn >= J.n_at;
+        return J;
+    };
+    tile_run<true, WIDE, 2, false, T, 2>(smem, share.count, job, [&](const UpJob &J, f32x4 (&acc)[T::TM][T::TN], char *buffer) {
+        const int n0 = J.n0, n_at = J.n_at, at0 = J.at0, block = J.block, lane = fresh(threadIdx.x) & 63, g = lane >> 4, i = lane & 15;
+        uint32_t *const most = reinterpret_cast<uint32_t *>(buffer + PLACES * BLOCK);          // [2 waves][PLACES], behind the tile's quantised rows
+        const bool whole = n0 + BLOCK <= ff;
+        uint32_t mine[T::TN];
 #pragma unroll
-    for (int j = 0; j < T::TN; j++) {
-        mine[j] = 0u;
+        for (int j = 0; j < T::TN; j++) {
+            mine[j] = 0u;
+            float v[16], u[16];
 #pragma unroll
-        for (int m = 0; m < 4; m++)
+            for (int k = 0; k < 16; k++) { v[k] = acc[k / 4][j][k % 4]; u[k] = acc[k / 4 + 4][j][k % 4]; }
+            gated_all(kind, limit, v, u);
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                float v = gated(kind, limit, acc[m][j][r], acc[m + 4][j][r]);
-                if (!whole && n0 + 64 * wm + 16 * m >= ff) v = 0.0f;          // (ff in whole 16s)
-                acc[m][j][r] = v;
-                mine[j] = dpp_max(mine[j], abs_bits(v));
+            for (int k = 0; k < 16; k++) {
+                if (!whole && n0 + 64 * wm + 16 * (k / 4) >= ff) v[k] = 0.0f;          // (ff in whole 16s)
+                acc[k / 4][j][k % 4] = v[k];
+                mine[j] = dpp_max(mine[j], abs_bits(v[k]));
             }
-        mine[j] = dpp_max(mine[j], (uint32_t)__shfl_xor((int)mine[j], 16, 64));
-        mine[j] = dpp_max(mine[j], (uint32_t)__shfl_xor((int)mine[j], 32, 64));
-        if (g == 0) most[wm * PLACES + MINE * wn + 16 * j + i] = mine[j];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < T::TN; j++) {
-        const int at = MINE * wn + 16 * j + i;
-        const float sc = scale_of(dpp_max(most[at], most[PLACES + at])), inv = 1.0f / sc;
-        if (wm == 0 && g == 0 && at < n_at) s[(size_t)(at0 + at) * fb + block] = sc;
-#pragma unroll
-        for (int m = 0; m < 4; m++) {
-            const float v[4] = {acc[m][j][0], acc[m][j][1], acc[m][j][2], acc[m][j][3]};
-            *reinterpret_cast<uint32_t *>(smem + at * BLOCK + 16 * ((4 * wm + m) ^ (at & 7)) + 4 * g) = quantise4(v, inv);
+            mine[j] = dpp_max(mine[j], (uint32_t)__shfl_xor((int)mine[j], 16, 64));
+            mine[j] = dpp_max(mine[j], (uint32_t)__shfl_xor((int)mine[j], 32, 64));
+            if (g == 0) most[wm * PLACES + MINE * wn + 16 * j + i] = mine[j];
         }
-    }
-    __syncthreads();
+        lds_barrier();
 #pragma unroll
-    for (int k = threadIdx.x; k < PLACES * 8; k += 64 * T::WAVES) {
-        const int at = k >> 3, piece = k & 7;
-        if (at < n_at && n0 + 16 * piece < ff) *reinterpret_cast<u32x4 *>(q + (size_t)(at0 + at) * ff + n0 + 16 * piece) = *reinterpret_cast<const u32x4 *>(smem + at * BLOCK + 16 * (piece ^ (at & 7)));
-    }
+        for (int j = 0; j < T::TN; j++) {
+            const int at = MINE * wn + 16 * j + i;
+            const float sc = scale_of(dpp_max(most[at], most[PLACES + at])), inv = 1.0f / sc;
+            if (wm == 0 && g == 0 && at < n_at) s[(size_t)(at0 + at) * fb + block] = sc;
+#pragma unroll
+            for (int m = 0; m < 4; m++) {
+                const float v[4] = {acc[m][j][0], acc[m][j][1], acc[m][j][2], acc[m][j][3]};
+                *reinterpret_cast<uint32_t *>(buffer + at * BLOCK + 16 * ((4 * wm + m) ^ (at & 7)) + 4 * g) = quantise4(v, inv);
+            }
+        }
+        lds_barrier();
+#pragma unroll
+        for (int k = fresh(threadIdx.x) & 511; k < PLACES * 8; k += 64 * T::WAVES) {
+            const int at = k >> 3, piece = k & 7;
+            if (at < n_at && n0 + 16 * piece < ff) *reinterpret_cast<u32x4 *>(q + (size_t)(at0 + at) * ff + n0 + 16 * piece) = *reinterpret_cast<const u32x4 *>(buffer + at * BLOCK + 16 * (piece ^ (at & 7)));
+        }
+    });
 }
 
 template <bool WIDE, int PLACES>
@@ -553,22 +575,26 @@ __global__ void __launch_bounds__(512, 2) k_moe_fp8_down_tile(const uint8_t *__r
     constexpr int MINE = 16 * T::TN;          // places of a wave
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1;
-    int tile, block;
-    if (!moe_tile(n_tiles, (width + 255) / 256, tile, block)) return;
-    const int e = tiles[3 * tile], at0 = tiles[3 * tile + 1], n_at = tiles[3 * tile + 2], n0 = block * 256;
-    f32x4 acc[T::TM][T::TN];
-#pragma unroll
-    for (int m = 0; m < T::TM; m++)
-#pragma unroll
-        for (int j = 0; j < T::TN; j++) acc[m][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int n = *n_tiles, blocks = (width + 255) / 256;
+    const Share share(n * blocks);
+    if (share.count == 0) return;
     const size_t wb = blocks_of(width), fb = blocks_of(ff);
-    const int nw = n0 + 128 * wm;
-    const float *sd = sdown + ((size_t)e * wb + min(nw, width - 1) / BLOCK) * fb;
-    tile_sums<WIDE, 1, true, T, 2>(
-        smem, ff, down + ((size_t)e * width + n0) * ff, [&](int r) { return (uint32_t)min(r, width - 1 - n0) * (uint32_t)ff; }, q + (size_t)at0 * ff,
-        [&](int r) { return (uint32_t)min(r, n_at - 1) * (uint32_t)ff; }, [&](int) { return sd; }, s + (size_t)(at0 + min(MINE * wn + lane % MINE, n_at - 1)) * fb, MINE * wn >= n_at || nw >= width, acc);
-    tile_out<T, 4>(smem, acc, [&](int t, int n, float *v) {
-        if (MINE * wn + t < n_at && nw + n < width) *reinterpret_cast<u32x4 *>(out + (size_t)(at0 + MINE * wn + t) * width + nw + n) = pack<IFA_F32>(v);          // (width in whole 16s)
+    auto job = [&](int k) {
+        DownJob J;
+        int tile, block;
+        moe_place(share.at(k), n, blocks, tile, block);
+        const int e = tiles[3 * tile], n0 = block * 256;
+        J.at0 = tiles[3 * tile + 1]; J.n_at = tiles[3 * tile + 2]; J.nw = n0 + 128 * wm; J.cols = ff; J.last_row = width - 1 - n0;
+        J.wbase = down + ((size_t)e * width + n0) * ff; J.abase = q + (size_t)J.at0 * ff;
+        J.sd = sdown + ((size_t)e * wb + min(J.nw, width - 1) / BLOCK) * fb;
+        J.sa = s + (size_t)(J.at0 + min(MINE * wn + (fresh(lane) & 63) % MINE, J.n_at - 1)) * fb;
+        J.idle = MINE * wn >= J.n_at || J.nw >= width;
+        return J;
+    };
+    tile_run<true, WIDE, 1, true, T, 2>(smem, share.count, job, [&](const DownJob &J, const f32x4 (&acc)[T::TM][T::TN], char *buffer) {
+        tile_out<T, true, 4>(buffer, acc, [&](int t, int n, float *v) {
+            if (MINE * wn + t < J.n_at && J.nw + n < width) *reinterpret_cast<u32x4 *>(out + (size_t)(J.at0 + MINE * wn + t) * width + J.nw + n) = pack<IFA_F32>(v);          // (width in whole 16s)
+        });
     });
 }
 
@@ -621,26 +647,24 @@ struct Work {
 };
 
 // Places of a tile: what takes least by these figures (us, measured: a step, that is a block of 128 columns, and beside the steps), with the experts' rows scattered about their mean as independent choices
-// would be.  A tile that is not full has waves that only fetch; they leave 0.4 of a step's time to those that do not.  us 128 / 192 / 256, rows: 64 experts of 2048 x 1408, top 6, 1024 164 / 173 / 181,
-// 1400 228 / 187 / 198, 2048 255 / 242 / 216, 3001 364 / 322 / 374, 4096 453 / 417 / 398; 8 of 4096 x 4096, top 2, 700 153 / 194 / 160, 1100 228 / 186 / 212; of these and six more the choice
-// is the fastest but for one (5 %).  exact: gate and up, wide: down on exact halves (256 places do not fit the registers then); 128 / 192, halves, 1400 rows 288 / 234, 2048 336 / 359, 3001 483 / 453, 32-bit
-// 316 / 245, 371 / 403, 532 / 477; of these and twelve more the choice is 0.9 % behind on average.
+// would be.  A tile that is not full has waves that only fetch; they leave 0.6 of a step's time to those that do not.  exact: gate and up, wide: down on exact halves.  us 128 / 192, rows: 64 experts of
+// 2048 x 1408, top 6, 1024 159 / 165, 1400 218 / 183, 2048 245 / 233, 2600 286 / 289, 3001 354 / 309, 4096 420 / 393; 8 of 4096 x 4096, top 2, 400 132 / 136, 1100 223 / 184; halves, 1024 186 / 209, 3001
+// 457 / 423; 32-bit 200 / 229, 496 / 456.  Of these and eighteen more the choice is 0.7 % behind the faster one on average.  (256 places spill registers in the ends of a tile: slower at all of them.)
 int places_for(int width, int ff, int experts, int pairs, bool exact, bool wide)
 {
-    constexpr struct { int places; double step, exact, beside; } FORMS[3] = {{128, 1.05, 1.7, 7.0}, {192, 1.40, 2.0, 8.0}, {256, 1.78, 0.0, 9.0}};
+    constexpr struct { int places; double step, exact, beside; } FORMS[2] = {{128, 1.1, 1.6, 5.5}, {192, 1.4, 2.1, 6.5}};
     constexpr double SHARE[7] = {0.07, 0.12, 0.20, 0.22, 0.20, 0.12, 0.07};          // of experts (k - 3) / 2 deviations from the mean
     const double mean = (double)pairs / experts;
     int best = 128;
     double least = 1e30;
     for (const auto &F : FORMS) {
-        if (exact && F.exact == 0.0) continue;
         double us = 0.0;
         for (int down = 0; down < 2; down++) {
             const double steps = (double)blocks_of(down ? ff : width), blocks = down ? (width + 255) / 256 : (double)blocks_of(ff), step = (down ? wide : exact) ? F.exact : F.step;
             double time = 0.0, tiles = 0.0;          // an expert's
             for (int k = 0; k < 7; k++) {
                 const double n = std::max(1.0, mean + 0.5 * (k - 3) * std::sqrt(mean)), full = std::floor(n / F.places), rest = n - full * F.places, live = std::ceil(4.0 * rest / F.places);
-                time += SHARE[k] * (full * (F.beside + steps * step) + (rest > 0.0 ? F.beside + steps * step * (0.6 + 0.1 * live) : 0.0));
+                time += SHARE[k] * (full * (F.beside + steps * step) + (rest > 0.0 ? F.beside + steps * step * (0.4 + 0.15 * live) : 0.0));
                 tiles += SHARE[k] * (full + (rest > 0.0 ? 1.0 : 0.0));
             }
             const double rounds = experts * tiles * blocks / 256, each = time / tiles;
@@ -722,23 +746,23 @@ int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t ld
         IFA_LAUNCH_CHECK();
         return IFA_OK;
     }
-    // lists go through an expert's matrices once for each 32 of its rows, tiles once for each 128 to 256 but with four launches more about them.  us lists / tiles, rows: 64 experts of 2048 x 1408, top 6,
+    // lists go through an expert's matrices once for each 32 of its rows, tiles once for each 128 or 192 but with four launches more about them.  us lists / tiles, rows: 64 experts of 2048 x 1408, top 6,
     // 64 126 / 141, 100 145 / 135, 256 235 / 145; 32 of 2048 x 704, top 4, 96 47 / 50, 160 58 / 51; 16 of 1024 x 704, top 4, 64 27 / 39, 128 39 / 40, 256 60 / 41; 8 of 4096 x 4096, top 2, 48 110 / 121, 64 135 / 120
     const bool many = pairs > LIST_MAX || ff > DOWN_FF || (double)pairs / experts >= (experts * bytes > 256e6 ? 12.0 : experts * bytes > 64e6 ? 15.0 : 30.0);
     if (many) {
         const int places = places_for(width, ff, experts, pairs, exact, wide), max_tiles = pairs / places + std::min(pairs, experts);
-        const int lds_bytes = places == 256 ? MoeTile<256>::SMEM : places == 192 ? MoeTile<192>::SMEM : MoeTile<128>::SMEM;
+        const int lds_bytes = places == 192 ? MoeTile<192>::SMEM : MoeTile<128>::SMEM;
         const size_t g_up = blocks_of(ff) * max_tiles, g_down = (size_t)((width + 255) / 256) * max_tiles;
         int *counts = (int *)(base + W.counts);
         hipLaunchKernelGGL(k_moe_fp8_count, dim3(W.blocks), dim3(1024), 0, st, idx_dev, pairs, experts, W.per, counts);
         hipLaunchKernelGGL(k_moe_fp8_place, dim3(W.blocks), dim3(1024), 0, st, idx_dev, pairs, experts, top, places, W.per, counts, place_row, pair_at, tiles, n_tiles);
-        const auto up_fn = exact ? (places == 192 ? k_moe_fp8_up_tile<true, 192> : k_moe_fp8_up_tile<true, 128>) : places == 256 ? k_moe_fp8_up_tile<false, 256> : places == 192 ? k_moe_fp8_up_tile<false, 192> : k_moe_fp8_up_tile<false, 128>;
-        const auto fn = wide ? (places == 192 ? k_moe_fp8_down_tile<true, 192> : k_moe_fp8_down_tile<true, 128>) : places == 256 ? k_moe_fp8_down_tile<false, 256> : places == 192 ? k_moe_fp8_down_tile<false, 192> : k_moe_fp8_down_tile<false, 128>;
+        const auto up_fn = places == 192 ? (exact ? k_moe_fp8_up_tile<true, 192> : k_moe_fp8_up_tile<false, 192>) : exact ? k_moe_fp8_up_tile<true, 128> : k_moe_fp8_up_tile<false, 128>;
+        const auto fn = places == 192 ? (wide ? k_moe_fp8_down_tile<true, 192> : k_moe_fp8_down_tile<false, 192>) : wide ? k_moe_fp8_down_tile<true, 128> : k_moe_fp8_down_tile<false, 128>;
         IFA_HIP_CHECK(hipFuncSetAttribute((const void *)up_fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes));
         IFA_HIP_CHECK(hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes));
-        hipLaunchKernelGGL(up_fn, dim3((unsigned)g_up), dim3(512), lds_bytes, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, (const uint8_t *)a_e4m3, lda,
+        hipLaunchKernelGGL(up_fn, dim3((unsigned)std::min<size_t>(g_up, 256)), dim3(512), lds_bytes, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, (const uint8_t *)a_e4m3, lda,
                            (const float *)a_scale_f32, lds, place_row, tiles, n_tiles, glu_kind, limit, q, s);
-        hipLaunchKernelGGL(fn, dim3((unsigned)g_down), dim3(512), lds_bytes, st, (const uint8_t *)down_e4m3, (const float *)down_scale_f32, width, ff, q, s, tiles, n_tiles, out);
+        hipLaunchKernelGGL(fn, dim3((unsigned)std::min<size_t>(g_down, 256)), dim3(512), lds_bytes, st, (const uint8_t *)down_e4m3, (const float *)down_scale_f32, width, ff, q, s, tiles, n_tiles, out);
     } else {
         hipLaunchKernelGGL(exact ? k_moe_fp8_up_list<true> : k_moe_fp8_up_list<false>, dim3(ff / 16, experts), dim3(64 * LIST_WAVES), 0, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, pairs, top,
                            (const uint8_t *)a_e4m3, lda, (const float *)a_scale_f32, lds, idx_dev, glu_kind, limit, act);

@@ -227,7 +227,8 @@ def check_product(c, want, bound, dtype, extra=0.0, loose=0.0):
 
 LINEAR_SHAPES = [(1, 16, 16), (1, 100, 144), (1, 4096, 512), (2, 33, 2064), (3, 257, 128), (4, 48, 4000), (5, 300, 1408), (8, 128, 256), (9, 1000, 272), (16, 64, 640), (17, 130, 912), (24, 704, 2064),
                  (33, 96, 384), (47, 1040, 1024), (64, 513, 144), (65, 257, 768), (100, 640, 400), (127, 384, 2048), (128, 128, 128), (129, 129, 144), (200, 1000, 1040), (256, 512, 256), (257, 300, 512),
-                 (300, 2050, 1408), (511, 1300, 656), (1030, 264, 1024), (40, 4096, 4096), (1500, 1552, 384)]
+                 (300, 2050, 1408), (511, 1300, 656), (1030, 264, 1024), (40, 4096, 4096), (1500, 1552, 384),
+                 (4100, 4400, 112), (4100, 4400, 144), (2100, 9000, 272), (3300, 8300, 2064)]          # (the last four: more tiles than workgroups)
 
 
 @pytest.mark.parametrize("tokens,rows,cols", LINEAR_SHAPES)
@@ -352,7 +353,7 @@ def expert_case(rows, width, ff, E, top, seed, dropped=0.0, one=False):
 
 EXPERT_SHAPES = [(1, 64, 48, 4, 2, 0), (1, 2048, 1408, 16, 6, 0), (2, 144, 128, 3, 3, 1), (3, 272, 400, 8, 1, 3), (5, 1024, 704, 32, 4, 0), (9, 400, 272, 5, 2, 1), (17, 512, 256, 4, 4, 2), (40, 256, 144, 60, 8, 0),
                  (53, 1040, 336, 8, 2, 3), (130, 384, 640, 3, 1, 0), (301, 528, 208, 6, 3, 1), (700, 256, 384, 2, 2, 0), (1100, 128, 128, 64, 5, 0),
-                 (1100, 528, 400, 64, 9, 0), (1500, 528, 400, 64, 9, 3)]          # (tiles of 192 and 256 places)
+                 (1100, 528, 400, 64, 9, 0), (1500, 528, 400, 64, 9, 3)]          # (tiles of 192 and of 128 places, more than workgroups)
 
 
 @pytest.mark.parametrize("rows,width,ff,E,top,kind", EXPERT_SHAPES)
