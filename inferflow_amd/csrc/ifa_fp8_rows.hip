@@ -4,7 +4,7 @@
 //   activation:  v = act(gate) * up
 // Both are bound by memory: a thread keeps its pieces of 16 bytes in registers, so that every value comes once and leaves once; a block of 128 columns
 // is 32 (32-bit) or 16 (16-bit values) neighbouring lanes, whose maximum takes four or five steps between lanes.
-// Measured: norm with the residual, 4096 x 4096 in 32 bits 48.4 us, 4.5 TB/s (a large copy: 4.9); activation, 2051 x 11008 bf16 22.7 us, 5.0 TB/s; few rows 2.5 us, a launch's start and end.
+// Measured: norm with the residual, 4096 x 4096 in 32 bits 45.3 us, 4.8 TB/s (a large copy: 4.9); activation, 2051 x 11008 bf16 22.7 us, 5.0 TB/s; few rows 2.5 us, a launch's start and end.
 #include "ifa_host.h"
 #include "ifa_fp8.h"
 
@@ -107,9 +107,12 @@ int norm_add(void *x, size_t ldx, size_t rows, size_t cols, const void *m, size_
 #define IFA_NORM(P)                                                                                                                                                        \
     hipLaunchKernelGGL((k_norm_add_fp8<DT, P>), dim3((unsigned)rows), dim3((unsigned)((pieces + 64 * P - 1) / (64 * P) * 64)), 0, s, (T *)x, ldx, (int)cols, (const T *)m, ldm, \
                        (const bf16_t *)w, w_offset, eps, (T *)h, ldh, (uint8_t *)q, ldq, (float *)scale, lds)
-    if (pieces <= 1024) IFA_NORM(1);
-    else if (pieces <= 2048) IFA_NORM(2);
-    else if (pieces <= 4096) IFA_NORM(4);
+    // threads of a row: few rows want all their requests at once, many rows several workgroups on a compute unit.  us 1024 / 512 at most, rows of 4096 32-bit columns: 4096 48.4 / 45.3, 1024 13.2 / 12.0,
+    // 512 7.7 / 7.6, 256 5.4 / 5.5, 1 3.3 / 3.6; 2048 rows of 8192 bf16 35.9 / 34.7, 64 5.1 / 5.2
+    const size_t most = rows > 512 ? 512 : 1024;
+    if (pieces <= most) IFA_NORM(1);
+    else if (pieces <= 2 * most) IFA_NORM(2);
+    else if (pieces <= 4 * most) IFA_NORM(4);
     else IFA_NORM(8);
 #undef IFA_NORM
     IFA_LAUNCH_CHECK();

@@ -88,7 +88,7 @@ def check_quantised(q, scale, v, rel):
 
 
 @pytest.mark.parametrize("dtype", [0, 1, 2])
-@pytest.mark.parametrize("rows,cols", [(1, 16), (3, 48), (2, 128), (5, 144), (1, 1040), (7, 2048), (2, 4112), (3, 8208), (1, 16400), (2, 32768), (300, 256), (33, 2832)])
+@pytest.mark.parametrize("rows,cols", [(1, 16), (3, 48), (2, 128), (5, 144), (1, 1040), (7, 2048), (2, 4112), (3, 8208), (1, 16400), (2, 32768), (300, 256), (33, 2832), (600, 4112), (513, 20016), (515, 32768)])
 @pytest.mark.parametrize("add,plain,weight", [(True, True, True), (False, False, True), (True, False, False)])
 def test_norm_with_the_residual(dtype, rows, cols, add, plain, weight):
     g, kind = gen(rows * 7 + cols), TYPES[dtype]
