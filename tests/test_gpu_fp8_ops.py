@@ -353,7 +353,8 @@ def expert_case(rows, width, ff, E, top, seed, dropped=0.0, one=False):
 
 EXPERT_SHAPES = [(1, 64, 48, 4, 2, 0), (1, 2048, 1408, 16, 6, 0), (2, 144, 128, 3, 3, 1), (3, 272, 400, 8, 1, 3), (5, 1024, 704, 32, 4, 0), (9, 400, 272, 5, 2, 1), (17, 512, 256, 4, 4, 2), (40, 256, 144, 60, 8, 0),
                  (53, 1040, 336, 8, 2, 3), (130, 384, 640, 3, 1, 0), (301, 528, 208, 6, 3, 1), (700, 256, 384, 2, 2, 0), (1100, 128, 128, 64, 5, 0),
-                 (1100, 528, 400, 64, 9, 0), (1500, 528, 400, 64, 9, 3)]          # (tiles of 192 and of 128 places, more than workgroups)
+                 (1100, 528, 400, 64, 9, 0), (1500, 528, 400, 64, 9, 3),
+                 (1100, 112, 144, 400, 2, 0), (1100, 272, 112, 400, 2, 1)]          # (the last four: tiles of 192 and of 128 places, more than workgroups, of one block and of several)
 
 
 @pytest.mark.parametrize("rows,width,ff,E,top,kind", EXPERT_SHAPES)
