@@ -120,7 +120,8 @@ template <int LANES> __device__ __forceinline__ uint32_t group_max(uint32_t v)
 // ---- products over one block of 128 columns.  Lane l holds 32 values of row l % 16 of either operand; which 32 of the block is free as long as both operands have the same (the sum does not
 // know their order); here columns 16 (l / 16) .. + 15 and those 64 further on.  The result: column l % 16 (an activation row), rows 4 (l / 16) .. + 3 (matrix rows).
 // Two forms.  v_mfma_f32_16x16x128_f8f6f4 adds eight products after shifting them to the exponent of the largest one, and what falls below 2^-13 of it is cut off (measured with pairs of products;
-// sums of unlike terms come out 1.5e-5 off, rms): enough in front of a rounding to 16 bits, not for a 32-bit result.  WIDE: the values as halves (exact: e4m3 fits) through four
+// sums of unlike terms come out 1.5e-5 off, rms): enough in front of a rounding to 16 bits, not for a 32-bit result, nor for sums that choose an e4m3 value each (experts' gate and up; v_mfma_f32_16x16x32_fp8_fp8
+// is off by as much).  WIDE: the values as halves (exact: e4m3 fits) through four
 // v_mfma_f32_16x16x32_f16, which keep 32-bit sums; half the rate, and a conversion for each two values.
 __device__ __forceinline__ i32x8 both_halves(u32x4 lo, u32x4 hi)
 {

@@ -159,9 +159,8 @@ __global__ void __launch_bounds__(64 * ROUTE_ROWS) k_moe_route_groups(const floa
 
 // ---- one to a few rows, two launches: every (row, choice) pair streams its expert's matrices.
 // act[p][n] = act(Gate_e a) (Up_e a) of pair p; grid (16 columns each, pairs), the blocks of columns shared out to the waves
-// Bound by the matrices' bytes and a launch's start and end: 6 experts of 2048 x 1408, 34.6 MB, 10.2 us (7.0 at a copy's rate).
+// Bound by the matrices' bytes and a launch's start and end: 6 experts of 2048 x 1408, 34.6 MB, 11.9 us (7.0 at a copy's rate; 10.2 with sums by the 8-bit instructions, see ifa_moe_experts_fp8).
 constexpr int PAIR_WAVES = 8;
-template <bool WIDE>
 __global__ void __launch_bounds__(64 * PAIR_WAVES) k_moe_fp8_up_pairs(const uint8_t *__restrict__ gu, const float *__restrict__ sgu, int width, int ff, int experts, int top,
                                                                       const uint8_t *__restrict__ a, size_t lda, const float *__restrict__ sa, size_t lds, const int *__restrict__ idx, int kind,
                                                                       float limit, float *__restrict__ act)
@@ -177,7 +176,7 @@ __global__ void __launch_bounds__(64 * PAIR_WAVES) k_moe_fp8_up_pairs(const uint
     const float *sar[1] = {sa + t * lds};
     f32x4 acc[2][1];
     acc[0][0] = acc[1][0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    stream_blocks<WIDE, 1, 2, 1>(wr, swr, ar, sar, width, wave, PAIR_WAVES, acc);
+    stream_blocks<true, 1, 2, 1>(wr, swr, ar, sar, width, wave, PAIR_WAVES, acc);
     join_waves<PAIR_WAVES, 2, 1>(acc, red);
     if (wave > 0 || (lane & 15)) return;          // (the sixteen activation rows of the products are one and the same)
     float v[4] = {acc[0][0][0], acc[0][0][1], acc[0][0][2], acc[0][0][3]};
@@ -304,7 +303,7 @@ template <int WAVES> __device__ __forceinline__ int list_pairs(const int *__rest
 
 // act[p] of the expert's pairs; grid (16 columns each, experts), the blocks of columns shared out to the waves.  (A workgroup of 128 columns, a wave 16 of them, could quantise them too: few workgroups,
 // 22.6 + 3.4 -> 32.5 us for 53 rows of four of 32 experts, 2048 x 704.)  Bound by the matrices' bytes, 92 MB there: 22 us, 4.2 TB/s.
-template <bool WIDE, int TILES>
+template <int TILES>
 __device__ __forceinline__ void up_list(const uint16_t *list, int n, const uint8_t *const (&wr)[2], const float *const (&swr)[2], int n0, int width, int ff, int top, const uint8_t *a, size_t lda,
                                         const float *sa, size_t lds, int kind, float limit, float *act, f32x4 *red)
 {
@@ -318,7 +317,7 @@ __device__ __forceinline__ void up_list(const uint16_t *list, int n, const uint8
         ar[j] = a + t * lda; sar[j] = sa + t * lds;
         acc[0][j] = acc[1][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    stream_blocks<WIDE, 1, 2, TILES, false>(wr, swr, ar, sar, width, wave, LIST_WAVES, acc);
+    stream_blocks<true, 1, 2, TILES, false>(wr, swr, ar, sar, width, wave, LIST_WAVES, acc);
     join_waves<LIST_WAVES, 2, TILES>(acc, red);
     if (wave == 0) {
 #pragma unroll
@@ -331,7 +330,6 @@ __device__ __forceinline__ void up_list(const uint16_t *list, int n, const uint8
     }
     __syncthreads();          // (`red` is read)
 }
-template <bool WIDE>
 __global__ void __launch_bounds__(64 * LIST_WAVES) k_moe_fp8_up_list(const uint8_t *__restrict__ gu, const float *__restrict__ sgu, int width, int ff, int pairs, int top,
                                                                      const uint8_t *__restrict__ a, size_t lda, const float *__restrict__ sa, size_t lds, const int *__restrict__ idx, int kind,
                                                                      float limit, float *__restrict__ act)
@@ -344,8 +342,8 @@ __global__ void __launch_bounds__(64 * LIST_WAVES) k_moe_fp8_up_list(const uint8
     const uint8_t *wr[2] = {gu + ((size_t)e * 2 * ff + r0) * width, gu + ((size_t)(e * 2 + 1) * ff + r0) * width};
     const float *swr[2] = {sgu + ((size_t)e * 2 * fb + n0 / BLOCK) * wb, sgu + ((size_t)(e * 2 + 1) * fb + n0 / BLOCK) * wb};
     for (int at = 0; at < n; at += 32) {
-        if (n - at <= 16) up_list<WIDE, 1>(list + at, n - at, wr, swr, n0, width, ff, top, a, lda, sa, lds, kind, limit, act, red);
-        else up_list<WIDE, 2>(list + at, n - at, wr, swr, n0, width, ff, top, a, lda, sa, lds, kind, limit, act, red);
+        if (n - at <= 16) up_list<1>(list + at, n - at, wr, swr, n0, width, ff, top, a, lda, sa, lds, kind, limit, act, red);
+        else up_list<2>(list + at, n - at, wr, swr, n0, width, ff, top, a, lda, sa, lds, kind, limit, act, red);
     }
 }
 
@@ -497,8 +495,8 @@ struct DownJob {
 };
 
 // a tile of 128 gate rows and the 128 up rows of the same columns: one block of the activations, which leave it quantised.  Bound by the products and a tile's ends (16 blocks of columns
-// between them): 17100 pairs of 64 experts, 2048 x 1408, 181 us
-template <bool WIDE, int PLACES>
+// between them): 17100 pairs of 64 experts, 2048 x 1408, 300 us (181 with sums by the 8-bit instructions, see ifa_moe_experts_fp8).  With 192 places eleven registers are laid aside for the ends of a tile, once a tile
+template <int PLACES>
 __global__ void __launch_bounds__(512, 2) k_moe_fp8_up_tile(const uint8_t *__restrict__ gu, const float *__restrict__ sgu, int width, int ff, const uint8_t *__restrict__ a, size_t lda,
                                                             const float *__restrict__ sa, size_t lds, const int *__restrict__ place_row, const int *__restrict__ tiles,
                                                             const int *__restrict__ n_tiles, int kind, float limit, uint8_t *__restrict__ q, float *__restrict__ s)
@@ -524,7 +522,7 @@ __global__ void __launch_bounds__(512, 2) k_moe_fp8_up_tile(const uint8_t *__res
         J.idle = MINE * wn >= J.n_at;
         return J;
     };
-    tile_run<true, WIDE, 2, false, T, 2>(smem, share.count, job, [&](const UpJob &J, f32x4 (&acc)[T::TM][T::TN], char *buffer) {
+    tile_run<true, true, 2, false, T, 2>(smem, share.count, job, [&](const UpJob &J, f32x4 (&acc)[T::TM][T::TN], char *buffer) {
         const int n0 = J.n0, n_at = J.n_at, at0 = J.at0, block = J.block, lane = fresh(threadIdx.x) & 63, g = lane >> 4, i = lane & 15;
         uint32_t *const most = reinterpret_cast<uint32_t *>(buffer + PLACES * BLOCK);          // [2 waves][PLACES], behind the tile's quantised rows
         const bool whole = n0 + BLOCK <= ff;
@@ -647,10 +645,11 @@ struct Work {
 };
 
 // Places of a tile: what takes least by these figures (us, measured: a step, that is a block of 128 columns, and beside the steps), with the experts' rows scattered about their mean as independent choices
-// would be.  A tile that is not full has waves that only fetch; they leave 0.6 of a step's time to those that do not.  exact: gate and up, wide: down on exact halves.  us 128 / 192, rows: 64 experts of
-// 2048 x 1408, top 6, 1024 159 / 165, 1400 218 / 183, 2048 245 / 233, 2600 286 / 289, 3001 354 / 309, 4096 420 / 393; 8 of 4096 x 4096, top 2, 400 132 / 136, 1100 223 / 184; halves, 1024 186 / 209, 3001
-// 457 / 423; 32-bit 200 / 229, 496 / 456.  Of these and eighteen more the choice is 0.7 % behind the faster one on average.  (256 places spill registers in the ends of a tile: slower at all of them.)
-int places_for(int width, int ff, int experts, int pairs, bool exact, bool wide)
+// would be.  A tile that is not full has waves that only fetch; they leave 0.6 of a step's time to those that do not.  step: by the 8-bit instructions (down, 16-bit outputs), exact: on exact
+// halves (gate and up; down, 32-bit outputs).  us 128 / 192, bfloat16 outputs, rows: 64 experts of 2048 x 1408, top 6, 1024 182 / 210, 1400 272 / 225, 2048 313 / 335, 2600 380 / 379, 3001 419 / 412, 4096
+// 540 / 508; 8 of 4096 x 4096, top 2, 400 140 / 156, 1100 293 / 233; 128 of 7168 x 2048, top 8, 600 1129 / 1274, 2048 2062 / 1865, 4096 3433 / 3231; 32-bit outputs, the first of these, 1024 200 / 229, 3001
+// 496 / 456.  At these eleven sizes of bfloat16 the choice is 0.7 % behind the faster one on average.
+int places_for(int width, int ff, int experts, int pairs, bool wide)
 {
     constexpr struct { int places; double step, exact, beside; } FORMS[2] = {{128, 1.1, 1.6, 5.5}, {192, 1.4, 2.1, 6.5}};
     constexpr double SHARE[7] = {0.07, 0.12, 0.20, 0.22, 0.20, 0.12, 0.07};          // of experts (k - 3) / 2 deviations from the mean
@@ -660,7 +659,7 @@ int places_for(int width, int ff, int experts, int pairs, bool exact, bool wide)
     for (const auto &F : FORMS) {
         double us = 0.0;
         for (int down = 0; down < 2; down++) {
-            const double steps = (double)blocks_of(down ? ff : width), blocks = down ? (width + 255) / 256 : (double)blocks_of(ff), step = (down ? wide : exact) ? F.exact : F.step;
+            const double steps = (double)blocks_of(down ? ff : width), blocks = down ? (width + 255) / 256 : (double)blocks_of(ff), step = down && !wide ? F.step : F.exact;
             double time = 0.0, tiles = 0.0;          // an expert's
             for (int k = 0; k < 7; k++) {
                 const double n = std::max(1.0, mean + 0.5 * (k - 3) * std::sqrt(mean)), full = std::floor(n / F.places), rest = n - full * F.places, live = std::ceil(4.0 * rest / F.places);
@@ -730,14 +729,14 @@ int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t ld
     uint8_t *q = base + W.q;
     const hipStream_t st = ifa_s(stream);
     const size_t few_lds = (size_t)2 * ((top + 1) / 2) * blocks_of(ff) * (BLOCK + 4);
-    // one or two rows, or up to four of small matrices: a stream for each pair.  us pairs / lists, rows x choices of experts, width x ff: 1 x 6 of 64, 2048 x 1408 20.6 / 33.5, 2 28.1 / 37.6, 4 48.4 / 47.8;
-    // 4 x 4 of 16, 1024 x 704 14.9 / 17.2, 8 25.5 / 18.4; 2 x 2 of 8, 4096 x 4096 54 / 55, 3 76 / 64
+    // one or two rows, or up to four of small matrices: a stream for each pair.  us pairs / lists, rows x choices of experts, width x ff: 1 x 6 of 64, 2048 x 1408 22.3 / 32.9, 2 31.3 / 40.5, 4 53.6 / 47.1;
+    // 4 x 4 of 16, 1024 x 704 15.9 / 16.8, 8 27.7 / 18.5; 2 x 2 of 8, 4096 x 4096 50 / 44, 3 71 / 56; 1 x 8 of 128, 7168 x 2048 85 / 105, 2 166 / 169, 3 246 / 223
     const double bytes = 3.0 * width * ff;
-    // Gate and up decide which e4m3 value an activation becomes: the 8-bit instructions' error moves one in some thousands to its neighbour, 1e-3 of the output.  That is below a bfloat16's rounding; for a half's
-    // or a 32-bit output both run on exact halves, gate and up for the former, down too for the latter (ifa_fp8.h).
-    const bool exact = y_dtype != IFA_BF16, wide = y_dtype == IFA_F32;
+    // Gate and up run on exact halves whatever the output's type (ifa_fp8.h): they decide which e4m3 value an activation becomes, and the 8-bit instructions' error would move one in some thousands to its
+    // neighbour, 1e-3 of the output and more -- as much as a bfloat16's rounding adds.  Down: on exact halves for a 32-bit output, by the 8-bit instructions in front of a rounding to 16 bits.
+    const bool wide = y_dtype == IFA_F32;
     if ((rows <= 2 || (rows <= 4 && bytes <= 4e6)) && few_lds <= 48 * 1024) {
-        hipLaunchKernelGGL(exact ? k_moe_fp8_up_pairs<true> : k_moe_fp8_up_pairs<false>, dim3(ff / 16, pairs), dim3(64 * PAIR_WAVES), 0, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, experts, top,
+        hipLaunchKernelGGL(k_moe_fp8_up_pairs, dim3(ff / 16, pairs), dim3(64 * PAIR_WAVES), 0, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, experts, top,
                            (const uint8_t *)a_e4m3, lda, (const float *)a_scale_f32, lds, idx_dev, glu_kind, limit, act);
 #define IFA_DOWN(DT) hipLaunchKernelGGL((k_moe_fp8_down_pairs<DT, 3>), dim3(width / 8, (unsigned)rows), dim3(64 * PAIR_WAVES), few_lds, st, (const uint8_t *)down_e4m3, (const float *)down_scale_f32, \
                                         width, ff, experts, top, act, idx_dev, (const float *)wgt_f32, (Elem<DT>::type *)y, ldy, accumulate)
@@ -746,17 +745,18 @@ int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t ld
         IFA_LAUNCH_CHECK();
         return IFA_OK;
     }
-    // lists go through an expert's matrices once for each 32 of its rows, tiles once for each 128 or 192 but with four launches more about them.  us lists / tiles, rows: 64 experts of 2048 x 1408, top 6,
-    // 64 126 / 141, 100 145 / 135, 256 235 / 145; 32 of 2048 x 704, top 4, 96 47 / 50, 160 58 / 51; 16 of 1024 x 704, top 4, 64 27 / 39, 128 39 / 40, 256 60 / 41; 8 of 4096 x 4096, top 2, 48 110 / 121, 64 135 / 120
+    // lists go through an expert's matrices once for each 32 of its rows, tiles once for each 128 or 192 but with two launches more about them.  us lists / tiles, rows: 64 experts of 2048 x 1408, top 6,
+    // 64 128 / 131, 100 139 / 131, 256 216 / 135; 32 of 2048 x 704, top 4, 96 45 / 52, 160 56 / 54; 16 of 1024 x 704, top 4, 64 27 / 38, 128 39 / 40, 256 59 / 45; 8 of 4096 x 4096, top 2, 48 110 / 120, 64 134 / 122;
+    // 128 of 7168 x 2048, top 8, 64 997 / 983, 128 1111 / 1001, 256 1457 / 1030
     const bool many = pairs > LIST_MAX || ff > DOWN_FF || (double)pairs / experts >= (experts * bytes > 256e6 ? 12.0 : experts * bytes > 64e6 ? 15.0 : 30.0);
     if (many) {
-        const int places = places_for(width, ff, experts, pairs, exact, wide), max_tiles = pairs / places + std::min(pairs, experts);
+        const int places = places_for(width, ff, experts, pairs, wide), max_tiles = pairs / places + std::min(pairs, experts);
         const int lds_bytes = places == 192 ? MoeTile<192>::SMEM : MoeTile<128>::SMEM;
         const size_t g_up = blocks_of(ff) * max_tiles, g_down = (size_t)((width + 255) / 256) * max_tiles;
         int *counts = (int *)(base + W.counts);
         hipLaunchKernelGGL(k_moe_fp8_count, dim3(W.blocks), dim3(1024), 0, st, idx_dev, pairs, experts, W.per, counts);
         hipLaunchKernelGGL(k_moe_fp8_place, dim3(W.blocks), dim3(1024), 0, st, idx_dev, pairs, experts, top, places, W.per, counts, place_row, pair_at, tiles, n_tiles);
-        const auto up_fn = places == 192 ? (exact ? k_moe_fp8_up_tile<true, 192> : k_moe_fp8_up_tile<false, 192>) : exact ? k_moe_fp8_up_tile<true, 128> : k_moe_fp8_up_tile<false, 128>;
+        const auto up_fn = places == 192 ? k_moe_fp8_up_tile<192> : k_moe_fp8_up_tile<128>;
         const auto fn = places == 192 ? (wide ? k_moe_fp8_down_tile<true, 192> : k_moe_fp8_down_tile<false, 192>) : wide ? k_moe_fp8_down_tile<true, 128> : k_moe_fp8_down_tile<false, 128>;
         IFA_HIP_CHECK(hipFuncSetAttribute((const void *)up_fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes));
         IFA_HIP_CHECK(hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes));
@@ -764,7 +764,7 @@ int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t ld
                            (const float *)a_scale_f32, lds, place_row, tiles, n_tiles, glu_kind, limit, q, s);
         hipLaunchKernelGGL(fn, dim3((unsigned)std::min<size_t>(g_down, 256)), dim3(512), lds_bytes, st, (const uint8_t *)down_e4m3, (const float *)down_scale_f32, width, ff, q, s, tiles, n_tiles, out);
     } else {
-        hipLaunchKernelGGL(exact ? k_moe_fp8_up_list<true> : k_moe_fp8_up_list<false>, dim3(ff / 16, experts), dim3(64 * LIST_WAVES), 0, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, pairs, top,
+        hipLaunchKernelGGL(k_moe_fp8_up_list, dim3(ff / 16, experts), dim3(64 * LIST_WAVES), 0, st, (const uint8_t *)gate_up_e4m3, (const float *)gate_up_scale_f32, width, ff, pairs, top,
                            (const uint8_t *)a_e4m3, lda, (const float *)a_scale_f32, lds, idx_dev, glu_kind, limit, act);
         const auto fn = wide ? k_moe_fp8_down_list<true> : k_moe_fp8_down_list<false>;
         const size_t list_lds = 16 * blocks_of(ff) * (BLOCK + 4);
