@@ -864,7 +864,8 @@ int ifa_moe_route_groups_f32(int score_kind, int groups, int groups_kept, int gr
 /* Gated experts over quantised rows: y[t] (+)= sum_k wgt[t][k] * Down_e q(f(Gate_e a[t], Up_e a[t])), e = idx[t][k], f as ifa_glu_fp8 (kinds 0 .. 3), q: quantised as above.  gate_up
  * [experts][gate ff | up ff][width] with scales [experts][2][ceil(ff / 128)][ceil(width / 128)], down [experts][width][ff] with scales [experts][ceil(width / 128)][ceil(ff / 128)].
  * idx outside 0 .. experts - 1 adds nothing; an expert may come more than once in a row.  width and ff in whole 16s; experts <= 1024, top <= 64, rows * top <= 1000000,
- * 2 ff width < 2^32 (the workspace of sizes beyond these: 0 bytes, and the call is refused).  idx_dev is read by more than one launch: it stays as it is until the call's work is done. */
+ * 2 ff width < 2^32 (the workspace of sizes beyond these: 0 bytes, and the call is refused).  idx_dev is read by more than one launch: it stays as it is until the call's work is
+ * done (a row whose choices change meanwhile is undefined; nothing outside the operands is read or written). */
 size_t ifa_moe_experts_fp8_workspace_bytes(size_t rows, int top, int width, int ff, int experts);
 int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t lda, const void *a_scale_f32, size_t lds, size_t rows, int width, int ff, int experts, int top,
                         const void *gate_up_e4m3, const void *gate_up_scale_f32, const void *down_e4m3, const void *down_scale_f32, const int *idx_dev, const void *wgt_f32, void *ws,

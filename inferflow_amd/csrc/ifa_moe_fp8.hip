@@ -409,16 +409,22 @@ __global__ void __launch_bounds__(64 * DOWN_WAVES) k_moe_fp8_down_list(const uin
     }
 }
 
-// ---- many rows: the pairs sorted by expert.  k_moe_fp8_count leaves, for each block of `per` pairs, how many of them chose each expert; k_moe_fp8_place adds these counts up and gives the pairs
-// their places: place_row[at] = the row of the pair at sorted place `at`, pair_at[p] = the place of pair p (-1: none), tiles = {expert, first place, places} of at most `tile` places of one
+// ---- many rows: the pairs sorted by expert.  k_moe_fp8_count leaves, for each block of `per` pairs, how many of them chose each expert, and in pair_at[p] the expert of pair p (-1: none); k_moe_fp8_place
+// adds these counts up and gives the pairs their places from what was counted (idx is looked at once: if it changed meanwhile, places counted by one idx and given out by another would run past the
+// lists): place_row[at] = the row of the pair at sorted place `at`, pair_at[p] = the place of pair p (-1: none), tiles = {expert, first place, places} of at most `tile` places of one
 // expert, *n_tiles.  (A workgroup alone took 31 us for 18000 pairs.)  A pair's place within its block's part of an expert's range is a matter of order alone: no value depends on it.
-__global__ void __launch_bounds__(1024) k_moe_fp8_count(const int *__restrict__ idx, int pairs, int experts, int per, int *__restrict__ counts)
+__global__ void __launch_bounds__(1024) k_moe_fp8_count(const int *__restrict__ idx, int pairs, int experts, int per, int *__restrict__ counts, int *__restrict__ pair_at)
 {
     __shared__ int cnt[1024];
     cnt[threadIdx.x] = 0;
     __syncthreads();
     const int p0 = blockIdx.x * per;
-    for (int p = p0 + threadIdx.x; p < min(p0 + per, pairs); p += 1024) { const int e = idx[p]; if (e >= 0 && e < experts) atomicAdd(&cnt[e], 1); }
+    for (int p = p0 + threadIdx.x; p < min(p0 + per, pairs); p += 1024) {
+        const int e = idx[p];
+        const bool known = e >= 0 && e < experts;
+        if (known) atomicAdd(&cnt[e], 1);
+        pair_at[p] = known ? e : -1;
+    }
     __syncthreads();
     if ((int)threadIdx.x < experts) counts[blockIdx.x * experts + threadIdx.x] = cnt[threadIdx.x];
 }
@@ -436,7 +442,7 @@ __device__ __forceinline__ int scan_1024(int v, int *part)
     __syncthreads();
     return in_front + x - v;
 }
-__global__ void __launch_bounds__(1024) k_moe_fp8_place(const int *__restrict__ idx, int pairs, int experts, int top, int tile, int per, const int *__restrict__ counts, int *__restrict__ place_row,
+__global__ void __launch_bounds__(1024) k_moe_fp8_place(int pairs, int experts, int top, int tile, int per, const int *__restrict__ counts, int *__restrict__ place_row,
                                                         int *__restrict__ pair_at, int *__restrict__ tiles, int *__restrict__ n_tiles)
 {
     __shared__ int cursor[1024], part[17], part2[17];
@@ -454,8 +460,8 @@ __global__ void __launch_bounds__(1024) k_moe_fp8_place(const int *__restrict__ 
     __syncthreads();
     const int p0 = blockIdx.x * per;
     for (int p = p0 + threadIdx.x; p < min(p0 + per, pairs); p += 1024) {
-        const int x = idx[p];
-        if (x < 0 || x >= experts) { pair_at[p] = -1; continue; }
+        const int x = pair_at[p];
+        if (x < 0) continue;
         const int at = atomicAdd(&cursor[x], 1);
         place_row[at] = p / top; pair_at[p] = at;
     }
@@ -754,8 +760,8 @@ int ifa_moe_experts_fp8(int glu_kind, float limit, const void *a_e4m3, size_t ld
         const int lds_bytes = places == 192 ? MoeTile<192>::SMEM : MoeTile<128>::SMEM;
         const size_t g_up = blocks_of(ff) * max_tiles, g_down = (size_t)((width + 255) / 256) * max_tiles;
         int *counts = (int *)(base + W.counts);
-        hipLaunchKernelGGL(k_moe_fp8_count, dim3(W.blocks), dim3(1024), 0, st, idx_dev, pairs, experts, W.per, counts);
-        hipLaunchKernelGGL(k_moe_fp8_place, dim3(W.blocks), dim3(1024), 0, st, idx_dev, pairs, experts, top, places, W.per, counts, place_row, pair_at, tiles, n_tiles);
+        hipLaunchKernelGGL(k_moe_fp8_count, dim3(W.blocks), dim3(1024), 0, st, idx_dev, pairs, experts, W.per, counts, pair_at);
+        hipLaunchKernelGGL(k_moe_fp8_place, dim3(W.blocks), dim3(1024), 0, st, pairs, experts, top, places, W.per, counts, place_row, pair_at, tiles, n_tiles);
         const auto up_fn = places == 192 ? k_moe_fp8_up_tile<192> : k_moe_fp8_up_tile<128>;
         const auto fn = places == 192 ? (wide ? k_moe_fp8_down_tile<true, 192> : k_moe_fp8_down_tile<false, 192>) : wide ? k_moe_fp8_down_tile<true, 128> : k_moe_fp8_down_tile<false, 128>;
         IFA_HIP_CHECK(hipFuncSetAttribute((const void *)up_fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes));
