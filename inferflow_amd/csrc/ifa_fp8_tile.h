@@ -21,16 +21,16 @@ typedef __attribute__((address_space(3))) char lds_char;
 // the products around it in their order; they have arrived behind arrive<n>() where n younger requests of the wave may be under way
 __device__ __forceinline__ void request16(const void *from, uint32_t to, int on)
 {
-    asm volatile("s_cmp_eq_u32 %2, 0\n\ts_cbranch_scc1 .Lrequest%=\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n.Lrequest%=:" ::"s"(to), "v"(from), "s"(__builtin_amdgcn_readfirstlane(on)) : "scc");
+    asm volatile("s_cmp_eq_u32 %2, 0\n\ts_cbranch_scc1 .Lrequest%=\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n.Lrequest%=:" ::"s"(to), "v"(from), "s"(__builtin_amdgcn_readfirstlane(on)) : "scc", "m0");
 }
 __device__ __forceinline__ void request16(const void *base, uint32_t offset, uint32_t to, int on)      // (base: the same in all lanes)
 {
     asm volatile("s_cmp_eq_u32 %3, 0\n\ts_cbranch_scc1 .Lrequest%=\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n.Lrequest%=:" ::"s"(to), "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(on))
-                 : "scc");
+                 : "scc", "m0");
 }
 __device__ __forceinline__ void request4(const void *from, uint32_t to, int on)      // 64 lanes' 4 bytes each to 256 bytes
 {
-    asm volatile("s_cmp_eq_u32 %2, 0\n\ts_cbranch_scc1 .Lrequest%=\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n.Lrequest%=:" ::"s"(to), "v"(from), "s"(__builtin_amdgcn_readfirstlane(on)) : "scc");
+    asm volatile("s_cmp_eq_u32 %2, 0\n\ts_cbranch_scc1 .Lrequest%=\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n.Lrequest%=:" ::"s"(to), "v"(from), "s"(__builtin_amdgcn_readfirstlane(on)) : "scc", "m0");
 }
 template <int N> __device__ __forceinline__ void arrive()      // this wave's requests but the last N, and everybody's; everybody's reads of LDS in front of it are done
 {
