@@ -852,6 +852,8 @@ int ifa_glu_fp8(int kind, float limit, int dtype, const void *gate_up, size_t ld
  * rounded once to c_dtype).  Products of a few hundred rows or less share their columns out to several workgroups through a workspace (16-byte aligned,
  * ifa_linear_fp8_workspace_bytes; 0: it is not used); with less, or none, they take longer and add up in another order.  tokens <= 1000000, rows < 2^26. */
 size_t ifa_linear_fp8_workspace_bytes(size_t rows, size_t cols, size_t tokens);
+/* which kernel a product takes with a workspace of ws_bytes (0: none): tiles of *tile_rows matrix rows x *tile_tokens rows, their columns shared out in *parts; *tile_rows 0: a stream of the matrix */
+int ifa_linear_fp8_plan(size_t rows, size_t cols, size_t lda, size_t tokens, int c_dtype, size_t ws_bytes, int *tile_rows, int *tile_tokens, int *parts);
 int ifa_linear_fp8(const void *w_e4m3, const void *w_scale_f32, size_t rows, size_t cols, const void *a_e4m3, size_t lda, const void *a_scale_f32, size_t lds, size_t tokens,
                    const void *bias_bf16, int accumulate, int c_dtype, void *c, size_t ldc, void *ws, size_t ws_bytes, ifa_stream stream);
 /* Router that chooses by groups: the n_all experts (at most 1024) are `groups` (at most 64) equal ranges.  score = softmax (score_kind 0) or sigmoid (1) of the logits, choice =

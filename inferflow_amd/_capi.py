@@ -233,6 +233,7 @@ SIGNATURES = {
     "ifa_norm_add_fp8": (_i, [_i, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _f, _f, _vp, _sz, _vp, _sz, _vp, _sz, _vp]),
     "ifa_glu_fp8": (_i, [_i, _f, _i, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _sz, _vp]),
     "ifa_linear_fp8_workspace_bytes": (_sz, [_sz, _sz, _sz]),
+    "ifa_linear_fp8_plan": (_i, [_sz, _sz, _sz, _sz, _i, _sz, _vp, _vp, _vp]),
     "ifa_linear_fp8": (_i, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _sz, _vp, _i, _i, _vp, _sz, _vp, _sz, _vp]),
     "ifa_moe_route_groups_f32": (_i, [_i, _i, _i, _i, _i, _f, _f, _vp, _sz, _sz, _i, _i, _vp, _vp, _vp, _vp]),
     "ifa_moe_experts_fp8_workspace_bytes": (_sz, [_sz, _i, _i, _i, _i]),

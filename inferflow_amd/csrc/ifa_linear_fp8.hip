@@ -202,9 +202,9 @@ constexpr TileCost TILE_COST[2][N_TILES] = {{{256, 256, 1, {1.78}, 9.0}, {256, 1
                                             {{256, 256, 0, {}, 0.0}, {256, 128, 1, {1.5}, 7.0}, {128, 128, 2, {1.0, 1.8}, 5.5}, {128, 64, 3, {0.65, 1.0, 1.75}, 5.5}, {128, 32, 3, {0.6, 0.9, 1.25}, 3.7}}};
 struct Plan { int form, parts; double us; };          // form: a tile, or -1: the stream
 
-Plan choose(bool wide, size_t rows, size_t cols, size_t tokens, size_t ws_bytes)
+Plan choose(bool wide, size_t rows, size_t cols, size_t lda, size_t tokens, size_t ws_bytes)
 {
-    if (tokens <= 16 || cols > (1u << 22)) return {-1, 1, 0.0};
+    if (tokens <= 16 || cols > (1u << 22) || lda > (1u << 22)) return {-1, 1, 0.0};          // (a tile's offsets have 32 bits)
     const double out = (double)tokens * rows;
     const size_t nb = blocks_of(cols);
     Plan best = {-1, 1, 2.3 + std::max(8.6e-4 * ((rows + 15) / 16) * ((tokens + 31) / 32) * nb, 0.14 * nb)};
@@ -223,11 +223,13 @@ Plan choose(bool wide, size_t rows, size_t cols, size_t tokens, size_t ws_bytes)
     return best;
 }
 
+bool sizes_known(size_t rows, size_t cols, size_t tokens) { return rows > 0 && cols > 0 && tokens > 0 && cols % 16 == 0 && rows < (1u << 26) && cols < (1u << 30) && tokens <= 1000000; }
+
 template <int DT>
 int linear(const Product &P, hipStream_t s)
 {
-    const Plan plan = choose(DT == IFA_F32, P.rows, P.cols, P.tokens, !P.ws || P.lda > (1u << 22) ? 0 : P.ws_bytes);
-    switch (P.lda > (1u << 22) ? -1 : plan.form) {          // (a tile's offsets have 32 bits)
+    const Plan plan = choose(DT == IFA_F32, P.rows, P.cols, P.lda, P.tokens, P.ws ? P.ws_bytes : 0);
+    switch (plan.form) {
     case T_256x256: if constexpr (DT != IFA_F32) return launch_tile<DT, 256, 256, 2, 4>(P, plan.parts, s); [[fallthrough]];
     case T_256x128: return launch_tile<DT, 256, 128, 2, 4>(P, plan.parts, s);
     case T_128x128: return launch_tile<DT, 128, 128, 2, 2>(P, plan.parts, s);
@@ -245,13 +247,25 @@ extern "C" {
 
 size_t ifa_linear_fp8_workspace_bytes(size_t rows, size_t cols, size_t tokens) 
 {
-    if (rows == 0 || cols == 0 || tokens == 0 || rows >= (1u << 26) || cols >= (1u << 30) || tokens > 1000000) return 0;
+    if (!sizes_known(rows, cols, tokens)) return 0;
     size_t most = 0;
     for (int wide = 0; wide < 2; wide++) {
-        const Plan plan = choose(wide, rows, cols, tokens, (size_t)256 << 20);
+        const Plan plan = choose(wide, rows, cols, cols, tokens, (size_t)256 << 20);
         if (plan.parts > 1) most = std::max(most, (size_t)plan.parts * tokens * rows * 4);
     }
     return most;
+}
+
+int ifa_linear_fp8_plan(size_t rows, size_t cols, size_t lda, size_t tokens, int c_dtype, size_t ws_bytes, int *tile_rows, int *tile_tokens, int *parts)
+{
+    IFA_REQUIRE(tile_rows && tile_tokens && parts, "ifa_linear_fp8_plan: null pointer");
+    if (!elem_known(c_dtype)) return ifa_fail(IFA_ERR_DTYPE, "ifa_linear_fp8_plan: output dtype %d (F32, F16 or BF16)", c_dtype);
+    IFA_REQUIRE(sizes_known(rows, cols, tokens) && lda >= cols && lda % 16 == 0, "ifa_linear_fp8_plan: %zu x %zu over %zu rows (columns in whole 16s)", rows, cols, tokens);
+    const Plan plan = choose(c_dtype == IFA_F32, rows, cols, lda, tokens, ws_bytes);
+    *tile_rows = plan.form < 0 ? 0 : TILE_COST[0][plan.form].bm;
+    *tile_tokens = plan.form < 0 ? 0 : TILE_COST[0][plan.form].bn;
+    *parts = plan.parts;
+    return IFA_OK;
 }
 
 int ifa_linear_fp8(const void *w_e4m3, const void *w_scale_f32, size_t rows, size_t cols, const void *a_e4m3, size_t lda, const void *a_scale_f32, size_t lds, size_t tokens,
@@ -259,7 +273,7 @@ int ifa_linear_fp8(const void *w_e4m3, const void *w_scale_f32, size_t rows, siz
 {
     IFA_REQUIRE(w_e4m3 && w_scale_f32 && a_e4m3 && a_scale_f32 && c, "ifa_linear_fp8: null pointer");
     if (!elem_known(c_dtype)) return ifa_fail(IFA_ERR_DTYPE, "ifa_linear_fp8: output dtype %d (F32, F16 or BF16)", c_dtype);
-    IFA_REQUIRE(rows > 0 && cols > 0 && tokens > 0 && cols % 16 == 0 && rows < (1u << 26) && cols < (1u << 30) && tokens <= 1000000, "ifa_linear_fp8: %zu x %zu over %zu rows (columns in whole 16s)", rows,
+    IFA_REQUIRE(sizes_known(rows, cols, tokens), "ifa_linear_fp8: %zu x %zu over %zu rows (columns in whole 16s)", rows,
                 cols, tokens);
     IFA_REQUIRE(lda >= cols && lda % 16 == 0 && lds >= blocks_of(cols) && ldc >= rows, "ifa_linear_fp8: row strides");
     IFA_REQUIRE((((uintptr_t)w_e4m3 | (uintptr_t)a_e4m3 | (uintptr_t)ws) & 15) == 0 && (((uintptr_t)w_scale_f32 | (uintptr_t)a_scale_f32) & 3) == 0 && ((uintptr_t)bias_bf16 & 1) == 0
