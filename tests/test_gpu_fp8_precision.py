@@ -1,8 +1,9 @@
-"""What the sums of the operators in 8-bit floating point hold: the experts' hidden activations, seen through a second matrix that is the identity."""
+"""What the sums of the experts in 8-bit floating point hold: their hidden activations, seen through a second matrix that is the identity, and the second product of these."""
 import pytest
 import torch
 
 from tests import fp8_oracle as orc
+from tests.fp8_plans import limit_32
 from tests.gpu_util import sync
 from tests.test_gpu_fp8_ops import F8, TYPES, experts, expert_case, gen
 
@@ -16,8 +17,8 @@ def identity_case(rows, width, ff, E, seed):
     return a, sa, gu, sgu, one, torch.ones(E, orc.blocks(ff), orc.blocks(ff), device="cuda"), idx, torch.ones(rows, 1, device="cuda")
 
 
-# rows: one and four choices as pairs, lists of one and of two tiles, tiles of 128 and of 192 places
-IDENTITY = [(1, 2048, 2048, 2), (4, 1024, 1024, 3), (40, 1040, 1040, 3), (200, 512, 512, 8), (700, 640, 640, 2), (1300, 384, 384, 1)]
+# one and four choices as pairs, lists, tiles of 128 places and (the last) of 192
+IDENTITY = [(1, 2048, 2048, 2), (4, 1024, 1024, 3), (40, 1040, 1040, 3), (200, 512, 512, 8), (700, 640, 640, 2), (1300, 384, 384, 1), (2600, 1152, 1152, 16)]
 
 
 @pytest.mark.parametrize("rows,width,ff,E", IDENTITY)
@@ -50,3 +51,23 @@ def test_hidden_activations_have_sums_of_32_bits(rows, width, ff, E):
     want = 448 * orc.scales(v)
     got = torch.stack([p.abs().amax(-1) for p in y.double().split(128, -1)], -1)
     assert float((got - want).norm()) <= 2.0 ** -20 * float(want.norm())
+
+
+@pytest.mark.parametrize("rows,width,ff,E", IDENTITY)
+@pytest.mark.parametrize("accumulate", [0, 1])
+def test_the_second_product_has_sums_of_32_bits_for_32_bit_outputs(rows, width, ff, E, accumulate):
+    """The hidden activations as the identity shows them (each one rounding, 2^-24, off) times another second matrix, in 64 bits; then a weight's product and an addition: three roundings beside a product's."""
+    a, sa, gu, sgu, one, sone, idx, wgt = identity_case(rows, width, ff, E, rows + 5)
+    hidden = torch.zeros(rows, width, device="cuda")
+    experts(0, a, sa, width, gu, sgu, one, sone, idx, wgt, 0, hidden, 0)
+    down, sdown = orc.matrix(width, ff, 9, count=E, std=ff ** -0.5)
+    wgt = torch.randn(rows, 1, generator=gen(2), device="cuda")
+    y0 = torch.randn(rows, width, generator=gen(3), device="cuda")
+    y = y0.clone()
+    experts(0, a, sa, width, gu, sgu, down, sdown, idx, wgt, 0, y, accumulate); sync()
+    want = torch.empty(rows, width, dtype=torch.float64, device="cuda")
+    for e in range(E):
+        t = (idx[:, 0] == e).nonzero()[:, 0]
+        want[t] = hidden[t].double() @ orc.matrix_values(down[e], sdown[e]).t() * wgt[t].double()
+    full = want + (y0.double() if accumulate else 0.0)
+    assert float((y.double() - full).norm()) <= (limit_32(orc.blocks(ff)) + 2 * 2.0 ** -24) * float(want.norm()) + 2.0 ** -24 * float(full.norm())
