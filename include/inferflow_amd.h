@@ -838,7 +838,10 @@ int ifa_moe_experts_routed_rows_f32(int score_kind, int renorm, float renorm_eps
 /* [rows][cols] (row-major, no padding) one for each 128 x 128 block ([ceil(rows / 128)][ceil(cols / 128)]); the last block of either may be a part   */
 /* of one.  Columns come in whole 16s, e4m3 rows start on 16 bytes.  A block's scale is max(max |v| / 448, 2^-126), its values e4m3(v / scale)        */
 /* (to nearest, ties to even; v times the 32-bit reciprocal of the scale).  A block that holds an infinity or a NaN stands for NaN in all its values. */
-/* Dtypes of rows that are not quantised: IFA_F32, IFA_F16 or IFA_BF16.  Sums, norms and activations are fp32.  Deterministic.                       */
+/* Dtypes of rows that are not quantised: IFA_F32, IFA_F16 or IFA_BF16.  Norms and activations are fp32, and so are the sums of products whose      */
+/* outputs are IFA_F32 and of the experts' gate and up.  16-bit outputs of ifa_linear_fp8 and of the experts' second product come from the 8-bit     */
+/* matrix instructions: of each eight products added up, what lies below 2^-13 of the largest one is dropped (at most 7 / 2^13 of their sizes,       */
+/* 1.5e-5 of a sum as a rule); blocks of 128 are added in fp32.  Deterministic.                                                                     */
 /* ======================================================================== */
 /* residual update, RMS norm and quantisation in one pass: x += m (m null: x as it is; the sum rounded to dtype), v = x / sqrt(mean(x^2) + eps) * (w_offset + w[c])
  * (w bf16 [cols], null: 0), (q, scale) = v quantised, h = v in dtype (nullable: what a router reads).  x, m and h [rows][ld*] of dtype, whole 16 bytes a row;
@@ -859,13 +862,13 @@ int ifa_linear_fp8(const void *w_e4m3, const void *w_scale_f32, size_t rows, siz
 /* Router that chooses by groups: the n_all experts (at most 1024) are `groups` (at most 64) equal ranges.  score = softmax (score_kind 0) or sigmoid (1) of the logits, choice =
  * score + correction[e] (fp32: a bias for balance moves in steps that a bfloat16 would lose; nullable); a group's value is the sum of its group_best (1 or 2) largest choices; the
  * groups_kept groups of largest value stay; of their experts the `top` (at most 64) largest choices are taken, in falling order, the lower index first on ties.  weight = score,
- * renorm != 0: score / (sum of the taken scores + renorm_eps) (0 if that is 0), times wgt_scale.  An expert whose logit is -inf or NaN (or whose choice is NaN) is never taken and adds
+ * renorm != 0: score / (sum of the taken scores + renorm_eps) (0 if that is 0), times wgt_scale.  An expert whose logit is -inf or NaN (or whose choice is) is never taken and adds
  * nothing to its group; what is left over of a row has idx -1 and weight 0.  Scores and choices are formed and compared in 64 bits.  idx_dev / wgt_f32: [rows][top]. */
 int ifa_moe_route_groups_f32(int score_kind, int groups, int groups_kept, int group_best, int renorm, float renorm_eps, float wgt_scale, const void *logits_f32, size_t ld, size_t rows, int n_all,
                              int top, const void *correction_f32, int *idx_dev, void *wgt_f32, ifa_stream stream);
 /* Gated experts over quantised rows: y[t] (+)= sum_k wgt[t][k] * Down_e q(f(Gate_e a[t], Up_e a[t])), e = idx[t][k], f as ifa_glu_fp8 (kinds 0 .. 3), q: quantised as above.  gate_up
  * [experts][gate ff | up ff][width] with scales [experts][2][ceil(ff / 128)][ceil(width / 128)], down [experts][width][ff] with scales [experts][ceil(width / 128)][ceil(ff / 128)].
- * idx outside 0 .. experts - 1 adds nothing; an expert may come more than once in a row.  width and ff in whole 16s; experts <= 1024, top <= 64, rows * top <= 1000000,
+ * The same activations for every y_dtype.  idx outside 0 .. experts - 1 adds nothing; an expert may come more than once in a row.  width and ff in whole 16s up to 65536; experts <= 1024, top <= 64, rows * top <= 1000000,
  * 2 ff width < 2^32 (the workspace of sizes beyond these: 0 bytes, and the call is refused).  idx_dev is read by more than one launch: it stays as it is until the call's work is
  * done (a row whose choices change meanwhile is undefined; nothing outside the operands is read or written). */
 size_t ifa_moe_experts_fp8_workspace_bytes(size_t rows, int top, int width, int ff, int experts);

@@ -66,3 +66,15 @@ def test_experts(rows, width, ff, E, top):
         want, bound = bounds[dtype == 0]
         check_product(y[:rows], want, bound, dtype, extra=2.0 ** -24 * (want.abs() + 8), loose=FLIPS)
         assert (y[rows] == 4.0).all()
+
+
+@pytest.mark.parametrize("bad", [-float("inf"), float("nan")])
+def test_experts_whose_correction_takes_them_out(bad):
+    """as if their logits were -inf: not taken, nothing added to their group (sigmoid scores, so that the others' stay)"""
+    z, out = torch.randn(50, 32, generator=torch.Generator().manual_seed(1)), [0, 5, 8, 9, 10, 11, 12, 13, 14, 15, 31]
+    corr = 0.1 * torch.randn(32, generator=torch.Generator().manual_seed(2))
+    masked, taken_out = z.clone(), corr.clone()
+    masked[:, out], taken_out[out] = -float("inf"), bad
+    a, b = (route(1, 4, 3, 2, True, 1e-20, 1.0, *args, 12) for args in ((z, taken_out), (masked, corr)))
+    sync()
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and not set(a[0].flatten().tolist()) & set(out)
