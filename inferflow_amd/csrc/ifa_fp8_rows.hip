@@ -4,7 +4,7 @@
 //   activation:  v = act(gate) * up
 // Both are bound by memory: a thread keeps its pieces of 16 bytes in registers, so that every value comes once and leaves once; a block of 128 columns
 // is 32 (32-bit) or 16 (16-bit values) neighbouring lanes, whose maximum takes four or five steps between lanes.
-// Measured: norm with the residual, 4096 x 4096 in 32 bits 45.3 us, 4.8 TB/s (a large copy: 4.9); activation, 2051 x 11008 bf16 22.7 us, 5.0 TB/s; few rows 2.5 us, a launch's start and end.
+// Measured: norm with the residual, 4096 x 4096 in 32 bits 44.5 us, 4.9 TB/s (a large copy: 4.9), 2048 x 8192 bf16 33.3 us, 3.5 TB/s (its weights come two bytes at a time behind the row's sum); activation, 2051 x 11008 bf16 22.7 us, 5.0 TB/s; few rows 2.5 us, a launch's start and end.
 #include "ifa_host.h"
 #include "ifa_fp8.h"
 

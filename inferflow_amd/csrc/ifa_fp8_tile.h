@@ -56,7 +56,7 @@ template <int BM, int BN, int WM, int WN> struct Tile {
 // Wave (wm, wn)'s products m = 0 .. TM - 1 have matrix rows wm BM / WM + 16 m on; NSC 2: in two halves, m < TM / 2 from the tile's rows wm BM / (2 WM) on, the others BM / 2 further on, with matrix scales of
 // their own.
 // MANY: the next tile's first block is asked for in front of done(), which has the second buffer to itself; its second block behind done().  Otherwise there is one tile, and done() has both buffers.  Experts' gate and up, 16 blocks, 5.5
-// tiles a workgroup: 208 -> 194 us; what hangs on the lane alone is computed anew in each of these parts (fresh): kept across the blocks' loop it would take 40 registers.
+// tiles a workgroup, with the 8-bit instructions: 208 -> 194 us; what hangs on the lane alone is computed anew in each of these parts (fresh): kept across the blocks' loop it would take 40 registers.
 // A block's products (each over the wave's TN activation tiles) run without a break from block to block: a product's sums are taken in front of the one that takes its registers, TN products later.  The
 // barrier at a block's end stands in front of its last product, whose operands are read by then: under it the next block's first operands come from LDS.
 template <bool MANY, bool WIDE, int NSC, bool A32, class T, int WM, class Jobs, class Done> __device__ __forceinline__ void tile_run(char *smem, int jobs, Jobs job, Done done)

@@ -194,7 +194,8 @@ int launch_tile(const Product &P, int parts, hipStream_t s)
 
 // ---- which kernel.  Up to 16 rows: the stream.  From there on what takes least by these figures (us, measured with weights from memory): a stream of 32 rows a workgroup 2.3 and 8.6e-4 for each
 // workgroup and block of columns, or 0.14 for each block; tiles a step (a block) and beside the steps, with one, two or three workgroups on a compute unit; parts of the columns the join and the
-// planes' way to memory and back.  Against the fastest of 14 choices at 33 sizes from 19 to 2385 rows, 258 to 15883 matrix rows, 128 to 11840 columns: 2.7 % behind on average.
+// planes' way to memory and back.  Against the fastest of 16 choices at 28 sizes from 19 to 2385 rows, 258 to 11008 matrix rows, 656 to 11840 columns, 16- and 32-bit outputs: 4.5 % behind on average, 30 %
+// at worst (19 rows, 258 x 11840, where the stream is taken for slower than it is).
 // 256 x 256 tiles of 32-bit outputs do not fit the registers.
 struct TileCost { int bm, bn, per_cu; double step[3], beside; };
 enum { T_256x256, T_256x128, T_128x128, T_128x64, T_128x32, N_TILES };

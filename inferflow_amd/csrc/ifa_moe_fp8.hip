@@ -15,7 +15,7 @@ namespace {
 // ---- the router.  One wave per row, four rows a workgroup; lane l holds the choices of experts l, l + 64, ...  Scores and choices in 64 bits: two experts whose choices differ by less than a 32-bit
 // rounding are told apart as the formula does.  Bound by instructions (64-bit exponentials and quotients, a maximum over the wave for each expert taken), not by the logits' bytes; so the
 // choices are kept as integers that order like them, and the maximum is one of their upper halves (a comparison of 32 bits a step between lanes) unless two are equal there.
-// 8191 rows of 256 experts, 8 of 4 groups of 8: 14.2 us (735 vector instructions a wave, issued in 70 % of its time; the logits alone take 2 us); one to 64 rows 3.4 us and the launch.
+// 8191 rows of 256 experts, 8 of 4 groups of 8: 14.2 us (735 vector instructions a wave, issued in three quarters of the busy cycles; the logits alone take 2 us); one to 64 rows 3.4 us and the launch.
 constexpr int ROUTE_ROWS = 4;
 
 __device__ __forceinline__ uint64_t order_of(double v)          // orders like v; 0: no choice
