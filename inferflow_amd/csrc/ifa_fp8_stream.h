@@ -58,6 +58,8 @@ __device__ __forceinline__ void stream_blocks(const uint8_t *const (&w)[MATS], c
         Group G[2];
         const int groups = (whole - first + DEPTH * step - 1) / (DEPTH * step);
         auto at = [&](int g) { return first + g * DEPTH * step; };
+        // The condition below always holds with DEPTH 1, and stays: without it hipcc 7.2 takes the second half of an 8-bit operand for one that nobody has written where it copies the operand behind the loop's
+        // requests (16-bit outputs; its assembly shows "kill: def" of registers by others), and the sums are wrong.
         auto go = [&](const Group &X, int g) {
 #pragma unroll
             for (int d = 0; d < DEPTH; d++) if (at(g) + d * step < whole) one(X.w[d], X.a[d], X.sw[d], X.sa[d]);

@@ -15,7 +15,7 @@ class Graph:
     """a captured call with a copy put behind its first kernel"""
 
     def __init__(self, call, dst, src):
-        self.hip = hip = C.CDLL("libamdhip64.so")
+        self.hip = hip = capi()          # (the HIP runtime that the library is linked to)
         self.stream, self.graph, self.run = torch.cuda.Stream(), C.c_void_p(), C.c_void_p()
         s = C.c_void_p(self.stream.cuda_stream)
         self.ok(hip.hipStreamBeginCapture(s, 2))          # (relaxed)
